@@ -52,8 +52,7 @@ extern "C" int neko_attn_diag_trace(void* buf) {
 #endif                       // sub-tiles, 2 operand fragments of one fixed query block (the LDS reads leave the loop), 4 no mask loads
 #define NEKO_ATTN_Q0(q0) ((NEKO_ATTN_ABL & 2) ? 0 : (q0))
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
-// Two fp32 values per issue slot (v_pk_fma_f32 / v_pk_mul_f32 / v_pk_add_f32, neko_common.h f32x2_v): these kernels are bound
-// by the VALU issue rate, and everything around the exponential that is plain arithmetic on an accumulator pair packs.
+// Pairs of fp32 values (neko_common.h f32x2_v); the library is built without the packed fp32 instructions, a pair is two issue slots.
 // bit `bit` of w sign-extended to a dword (all ones / zero) in ONE instruction; written as asm because the compiler turns
 // `x & sbfe(w, bit, 1)` into v_and + v_cmp + v_cndmask
 template <typename T = void>
@@ -119,14 +118,12 @@ __device__ __forceinline__ uint32_t quad_bcast(uint32_t x, int i) {   // value o
 // ---- dropout keep decisions computed ONCE (forward) and reused by both backward kernels ------------------------------
 // The forward kernel's compare "hash byte >= threshold" for accumulator register r lands in an SGPR pair: a 64-bit lane
 // mask whose low word is {keep(query q0 + l, key k0 + c(r))}_l and whose high word is the same for key k0 + c(r) + 4
-// (c(r) = (r & 3) + 8 (r >> 2)).  Those 16 pairs = 32 dwords per 32 x 32 sub-tile are written with scalar stores
-// (s_store_dwordx4: wave-uniform data never touches a VGPR) to   mask[(b*H + h)][query block][key block][32]   and
+// (c(r) = (r & 3) + 8 (r >> 2)).  Those 16 pairs = 32 dwords per 32 x 32 sub-tile are gathered
+// into one VGPR (dword i in lane i, v_writelane) and leave in ONE 128-byte vector store to   mask[(b*H + h)][query block][key block][32]   and
 //   * dQ (same lane = query geometry) reads them back with scalar loads and applies each as the SGPR-pair operand of ONE
 //     v_cndmask_b32 -- instead of 10 VALU per hash word + compare + select per element;
 //   * dK/dV (lane = key) loads, per lane, the dword of ITS key (bits = the 32 queries of the block) and tests bit
 //     c(r) + 4 (lane / 32) with one v_bfe_i32 per register.
-// tools/probe/sstore_probe.hip checks the scalar-store / scalar-load round trip across kernels on gfx950.
-typedef uint32_t u32x4_s __attribute__((ext_vector_type(4)));
 // loads through the constant address space with a wave-uniform address are always scalar loads (s_load_dwordx*); through a
 // plain global pointer hipcc only selects them when it can prove that no store of the kernel may alias
 typedef __attribute__((address_space(4))) const unsigned long long const_u64;
@@ -135,11 +132,17 @@ __device__ __forceinline__ const void* uniform_ptr(const void* p) {
   return reinterpret_cast<const void*>(((uintptr_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32)) << 32) |
                                        (uintptr_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a));
 }
-// two lane masks -> 16 bytes at base + OFF (base wave-uniform, in SGPRs)
-template <int OFF>
-__device__ __forceinline__ void sstore_masks(uint32_t* base, unsigned long long m0, unsigned long long m1) {
-  const u32x4_s q = {(uint32_t)m0, (uint32_t)(m0 >> 32), (uint32_t)m1, (uint32_t)(m1 >> 32)};
-  asm volatile("s_store_dwordx4 %0, %1, %2" ::"s"(q), "s"(base), "n"(OFF) : "memory");
+// v_writelane_b32 (no clang builtin; the intrinsic, unlike inline asm, lets the compiler place the wait states behind the compare that wrote the mask)
+__device__ int amdgcn_writelane(int value, int lane, int old) __asm("llvm.amdgcn.writelane.i32");
+// the 16 lane masks of a sub-tile as one dword per lane: lane 2 i holds the low half of km[i], lane 2 i + 1 the high half (lanes >= 32: 0)
+__device__ __forceinline__ uint32_t masks_to_lanes(const unsigned long long (&km)[16]) {
+  int v = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    v = amdgcn_writelane((int)(uint32_t)km[i], 2 * i, v);
+    v = amdgcn_writelane((int)(uint32_t)(km[i] >> 32), 2 * i + 1, v);
+  }
+  return (uint32_t)v;
 }
 // position of key `kl` (0..31) of a sub-tile inside its 32 dwords: pair r = (kl & 3) + 4 (kl >> 3), half (kl >> 2) & 1
 __device__ __forceinline__ int mask_slot_of_key(int kl) { return 2 * ((kl & 3) + 4 * (kl >> 3)) + ((kl >> 2) & 1); }
@@ -412,17 +415,9 @@ __global__ __launch_bounds__(1024) void attn_fwd_res_kernel(const bf16_t* __rest
             st[4 * j + e] = keep ? st[4 * j + e] : 0.f;
           }
         }
-        if (MASK) {     // the sub-tile's 16 lane masks -> mask[(b*H+h)][qb][kbk][32 dwords], 8 scalar stores
-          uint32_t* mp = const_cast<uint32_t*>(static_cast<const uint32_t*>(
-              uniform_ptr(dmask + sg.mask0 + ((long)qb * nblk + kbk) * 32)));
-          sstore_masks<0>(mp, km[0], km[1]);
-          sstore_masks<16>(mp, km[2], km[3]);
-          sstore_masks<32>(mp, km[4], km[5]);
-          sstore_masks<48>(mp, km[6], km[7]);
-          sstore_masks<64>(mp, km[8], km[9]);
-          sstore_masks<80>(mp, km[10], km[11]);
-          sstore_masks<96>(mp, km[12], km[13]);
-          sstore_masks<112>(mp, km[14], km[15]);
+        if (MASK) {     // the sub-tile's 16 lane masks -> mask[(b*H+h)][qb][kbk][32 dwords], one 128-byte store
+          const uint32_t mv = masks_to_lanes(km);
+          if (lane < 32) dmask[sg.mask0 + ((long)qb * nblk + kbk) * 32 + lane] = mv;
         }
       }
 #pragma unroll
@@ -444,8 +439,6 @@ __global__ __launch_bounds__(1024) void attn_fwd_res_kernel(const bf16_t* __rest
       if (lane < 32) lse[sg.hrow + q] = m_run * LN2 + __logf(l_tot);
     }
   }
-  if (DROP && MASK)   // scalar stores sit in the scalar data cache until written back
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_dcache_wb\n\ts_waitcnt lgkmcnt(0)" ::: "memory");
 }
 
 // =====================================================================================================
