@@ -24,7 +24,10 @@ HEADERS = ["neko_common.h", "neko_kernels.h", os.path.join("..", "..", "include"
 EXTRA_DEPS = {"gemm_glds.hip": ["gemm_epi.h"], "gemm_a16.hip": ["gemm_epi.h", "gemm_a16_loop.inc"],
               "gemm_b16.hip": ["gemm_epi.h", "gemm_b16_loop.inc"], "gemm_p16.hip": ["gemm_epi.h", "gemm_p16_loop.inc"]}
 ARCH = "gfx950"
-FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-ffp-contract=on", "-Wno-unused-result"]
+FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-ffp-contract=on", "-Wno-unused-result",
+         # no packed fp32 instructions: hipcc forms them from ordinary float code by itself, and some of their forms have given wrong
+         # results on this hardware (the host pass of hipcc warns that it does not know the feature: harmless)
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 FLAGS += os.environ.get("NEKO_EXTRA_HIPCC_FLAGS", "").split()
 
 

@@ -86,10 +86,9 @@ __device__ __forceinline__ float gelu_grad_f(float x) {
   return fmaf(x * 0.39894228040143267794f, e, 0.5f * (1.0f + er));
 }
 
-// Two elements at a time on the packed fp32 pipe (v_pk_fma_f32 / v_pk_mul_f32: two lanes' worth of fp32 per issue slot):
-// the GEMM epilogues with GELU / GELU' are VALU-bound (256 x 256 results x ~16 slots each per tile against a 24-k-tile
-// main loop), and everything in the formulas above except v_rcp / v_exp / the sign transfer packs.  Same series, same
-// constants; gelu is rearranged so that the sign never has to be transferred:
+// Two elements at a time: one evaluation of the series for a pair of values.  (The pair type once selected the packed fp32
+// instructions; the library is built without them, see neko_amd/build.py, so a pair costs two full-rate issue slots per operation.)
+// Same series, same constants; gelu is rearranged so that the sign never has to be transferred:
 //   gelu(x)  = x/2 + |x|/2 * m,              m = 1 - poly(t) e   (erf(|z|))
 //   gelu'(x) = 1/2 + copysign(m/2, x) + x e / sqrt(2 pi)
 typedef float f32x2_v __attribute__((ext_vector_type(2)));
