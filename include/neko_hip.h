@@ -355,6 +355,53 @@ int neko_patch_pos_add_bwd_sorted(const float* dout, const int* hkeys_sorted, co
                                   const int* widx_sorted, float* d_row_emb, float* d_col_emb, int P, int d, int nrows, void* workspace,
                                   long ws_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Serving: an 8-bit key / value cache, attention over it, verification of drafted tokens; training: distillation from a teacher's top
+ * logits.  (Additions to v19: no earlier entry changes.)
+ *
+ * The cache of one layer holds nseq sequences x H key heads x cap positions (cap a multiple of 64) of hd = 32 / 64 / 128 channels in one
+ * byte a value, dtype 0 = e4m3 (OCP), 1 = int8, and one fp32 power-of-two scale per `block` (16 / 32 / 64) positions and head:
+ *   k8 [nseq][H][cap][hd]    v8 [nseq][H][cap / 16][hd][16]    k_scale, v_scale [nseq][H][cap / block]      value = code * scale
+ * Positions live in DEVICE memory (pos, n_new, length: int32 [nseq]), so that every launch is independent of them and can be captured.
+ *
+ * neko_kv8_append: rows 0 .. n-1 of k / v (bf16; element (s, t, h, c) at s * ss + t * st + h * hd + c; strides multiples of 8, 16-byte
+ *   aligned) go to positions pos[s] .. pos[s] + n - 1, n = min(n_new[s], T, cap - pos[s]) (n_new NULL: T).  A sequence with n <= 0, pos < 0
+ *   or pos >= cap is left alone, and so is every byte behind the new rows.  A block that holds older rows keeps its scale or gets a larger
+ *   one, and then its older codes are rounded again; a block without older rows starts afresh: setting pos back drops rows.  NaN is stored
+ *   as 0, magnitudes above 1.75 2^127 (infinities among them) as 1.75 2^127.
+ * neko_kv8_read: rows 0 .. L-1 of every sequence as bf16 (exact), k, v contiguous [nseq][L][H][hd]; rows t >= length[s] are written as 0.
+ * neko_attn_kv8: T rows a sequence at positions pos[s] + i (i < n as above; other rows of `out` are left as they are), G query heads per key
+ *   head (query head h * G + g reads key head h), q and out bf16 with strides as k above.  Row at position p sees t with start[s] <= t <= p and,
+ *   where window > 0, t > p - window or t < start[s] + sinks (start NULL: 0).  A row that sees nothing is 0.  `scale` multiplies q . k.
+ *   What lies in the cache outside [start, last row] never reaches the output.  max_len: host-known bound on pos + T (0: cap); it sizes
+ *   the split of the key axis and changes no result beyond rounding.  ws: neko_attn_kv8_ws_floats(..) floats (may be 0), private to the call.
+ * neko_verify_draft: sequence b, K + 1 rows of target logits (element (b, i, v) at b * t_sb + i * t_sr + v; fp32 or bf16), n = n_draft[b] <= K
+ *   drafted tokens [B][K] (n_draft NULL: K), draft logits in the same way or NULL (the draft was certain), u [B][K], r [B] in [0, 1).
+ *   With p_i, q_i the softmax at `temperature`: token i is kept while u_i q_i(x_i) < p_i(x_i); the token behind the `accepted` kept ones is the
+ *   smallest v whose cumulative weight exceeds r times the total, weights max(p - q, 0) of the first row not kept (p where nothing is left),
+ *   or p of row n.  temperature 0: kept while x_i is the row's largest logit (lowest index among equals), then the row's largest.
+ *   out_tokens [B][K + 1]: the kept tokens, the next one, then -1.  NaN logits count as -inf; a row without a logit above -inf keeps
+ *   nothing and gives the token -1.  K <= 62.
+ * neko_distill_topk: rows of R student logits z (fp32 or bf16, leading dimension ldz, columns >= V ignored) against k teacher logits and their
+ *   indices (t_val, t_idx [R][k]; an index outside [0, V) is no entry; equal indices add up):
+ *     loss_row = (1 - hard) tau^2 KL(softmax(t / tau) || softmax(z / tau)) + hard CE(z, target)      (target int64 [R], < 0: no such term)
+ *     dlogits  = weight[r] d loss_row / dz in z's type, 0 in columns V .. Vpad-1; may be z itself; NULL: loss only
+ *   weight 0: loss 0, gradient 0.  k <= 1024; Vpad, ldz, ldd multiples of 16 bytes. */
+int neko_kv8_append(void* k8, void* v8, float* k_scale, float* v_scale, int dtype, int nseq, int H, int cap, int hd, int block, const uint16_t* k,
+                    long k_ss, long k_st, const uint16_t* v, long v_ss, long v_st, const int* pos, const int* n_new, int T, void* stream);
+int neko_kv8_read(const void* k8, const void* v8, const float* k_scale, const float* v_scale, int dtype, int nseq, int H, int cap, int hd,
+                  int block, const int* length, int L, uint16_t* k, uint16_t* v, void* stream);
+long neko_attn_kv8_ws_floats(int nseq, int H, int G, int cap, int hd, int T, int max_len);
+int neko_attn_kv8(const void* k8, const void* v8, const float* k_scale, const float* v_scale, int dtype, int nseq, int H, int cap, int hd, int block,
+                  const uint16_t* q, long q_ss, long q_st, uint16_t* out, long o_ss, long o_st, int G, int T, const int* pos, const int* n_new,
+                  const int* start, int window, int sinks, float scale, int max_len, float* ws, long ws_floats, void* stream);
+long neko_verify_draft_ws_bytes(int B, int K, int V);
+int neko_verify_draft(const void* target, long t_sb, long t_sr, const void* draft, long d_sb, long d_sr, int is_bf16, int B, int K, int V,
+                      const long long* tokens, const float* u, const float* r, const int* n_draft, float temperature, int* accepted,
+                      long long* out_tokens, void* ws, long ws_bytes, void* stream);
+int neko_distill_topk(const void* z, long ldz, int is_bf16, int R, int V, int Vpad, const float* t_val, const int* t_idx, int k,
+                      const float* weight, float tau, const long long* target, float hard, float* loss_row, void* dlogits, long ldd, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

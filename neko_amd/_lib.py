@@ -69,6 +69,13 @@ SIGNATURES = {
     "neko_patch_pos_add_bwd_sorted": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _l, _vp],
     "neko_patch_pos_add": [_vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
     "neko_patch_pos_add_bwd": [_vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
+    "neko_kv8_append": [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _l, _l, _vp, _l, _l, _vp, _vp, _i, _vp],
+    "neko_kv8_read": [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _i, _vp, _vp, _vp],
+    "neko_attn_kv8_ws_floats": [_i, _i, _i, _i, _i, _i, _i],
+    "neko_attn_kv8": [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _l, _l, _vp, _l, _l, _i, _i, _vp, _vp, _vp, _i, _i, _f, _i, _vp, _l, _vp],
+    "neko_verify_draft_ws_bytes": [_i, _i, _i],
+    "neko_verify_draft": [_vp, _l, _l, _vp, _l, _l, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _f, _vp, _vp, _vp, _l, _vp],
+    "neko_distill_topk": [_vp, _l, _i, _i, _i, _i, _vp, _vp, _i, _vp, _f, _vp, _f, _vp, _vp, _l, _vp],
     "neko_abi_version": [],
 }
 
@@ -102,6 +109,8 @@ def load() -> C.CDLL:
     lib.neko_patch_pos_add_bwd_det_ws_bytes.restype = C.c_long
     lib.neko_pack_embed_bwd_sorted_ws_bytes.restype = C.c_long
     lib.neko_patch_pos_add_bwd_sorted_ws_bytes.restype = C.c_long
+    lib.neko_attn_kv8_ws_floats.restype = C.c_long
+    lib.neko_verify_draft_ws_bytes.restype = C.c_long
     lib.neko_status_string.argtypes = [_i]
     lib.neko_status_string.restype = C.c_char_p
     _lib = lib

@@ -1,0 +1,382 @@
+// Attention of T new rows per sequence over the 8-bit cache (layout: kv8.h).
+//
+//   out[s, i, hq] = sum_t softmax_t(scale * q[s, i, hq] . K[s, hq / G, t]) V[s, hq / G, t]   over the visible t of the row at position p = pos[s] + i:
+//   start[s] <= t <= p   and   (window == 0, or t > p - window, or t < start[s] + sinks)
+//
+// Rows i >= n_new[s] are left as they are; a row that sees nothing is 0.  Codes are unpacked to bf16 (exact), scores, maxima, sums and the
+// output accumulate in fp32; block scales never touch an operand: K's multiplies the scores, V's the probabilities.
+#include "kv8.h"
+
+namespace {
+
+struct AttnArgs {
+  const uint8_t *k8, *v8;
+  const float *ks, *vs;
+  const bf16_t* q;
+  bf16_t* out;
+  long q_ss, q_st, o_ss, o_st;
+  const int *pos, *n_new, *start;
+  float *part_o, *part_ml;           // [S * H][splits][row tiles * rows per tile][hd] and [..][2]
+  int S, H, G, cap, T, bshift, window, sinks, splits, rtiles;
+  float scale_log2e;
+};
+
+// What the rows of one tile see of their sequence.  Key tiles of 64 positions: first those with sinks, then the window (or everything).
+struct Span {
+  int rows;          // rows of this call (n * G)
+  int p0;            // position of row 0
+  int first;         // first visible key
+  int plast;         // last position of the tile's rows
+  int pfirst;        // first position of the tile's rows
+  int a0, na, b0, nt;
+};
+__device__ __forceinline__ bool span_of(const AttnArgs& a, int s, int r0, int r1, Span& sp) {
+  const int p = a.pos[s];
+  int n = min(a.n_new ? a.n_new[s] : a.T, a.T);
+  if (p < 0 || p >= a.cap || n <= 0) return false;
+  n = min(n, a.cap - p);
+  sp.rows = n * a.G;
+  if (r0 >= sp.rows) return false;
+  sp.p0 = p;
+  sp.pfirst = p + r0 / a.G;
+  sp.plast = p + (min(r1, sp.rows) - 1) / a.G;
+  sp.first = a.start ? max(a.start[s], 0) : 0;
+  if (sp.first > sp.plast) { sp.a0 = sp.na = sp.b0 = sp.nt = 0; return true; }
+  int lo = sp.first;
+  if (a.window > 0 && sp.pfirst - a.window + 1 > lo) lo = sp.pfirst - a.window + 1;
+  sp.b0 = lo >> 6;
+  const int nb = (sp.plast >> 6) + 1 - sp.b0;
+  sp.a0 = sp.first >> 6;
+  sp.na = 0;
+  if (a.window > 0 && a.sinks > 0) {
+    const int sink_last = (int)min((long)sp.first + a.sinks - 1, (long)sp.plast);
+    sp.na = max(0, min((sink_last >> 6) + 1, sp.b0) - sp.a0);
+  }
+  sp.nt = sp.na + nb;
+  return true;
+}
+__device__ __forceinline__ int tile_of(const Span& sp, int i) { return i < sp.na ? sp.a0 + i : sp.b0 + i - sp.na; }
+__device__ __forceinline__ bool visible(const AttnArgs& a, const Span& sp, int key, int p) {
+  return key <= p && key >= sp.first && (a.window == 0 || key > p - a.window || key < (long)sp.first + a.sinks);
+}
+
+// ---- few rows: a wave owns whole key tiles --------------------------------------------------------------------------------
+// One workgroup of NW waves per (split, head, sequence, row tile).  A wave takes every NW-th 64-key tile of its split and keeps its own
+// running maximum, sum and output for 16 NQ rows; the waves meet once at the end in LDS, the splits in a second kernel.  No LDS and no
+// barrier in the loop: operands go from memory to registers in matrix-operand order.  S^T = K Q^T (a lane holds 4 keys of one row per
+// 16 x 16 tile); the keys a matrix row stands for are chosen so that a lane's 16 scores of a 64-key tile are 16 CONSECUTIVE positions:
+// matrix row r of tile t is key 16 (r / 4) + 4 t + r % 4.  They are then, as they stand, the operand of O^T = V^T P^T whose other
+// operand is one 16-byte load of V's transposed tile, and they share one block scale.
+constexpr int KT = 64;
+
+template <int HD, int DT, int NQ, int NW>
+__global__ __launch_bounds__(NW * 64) void attn_kv8_rows_kernel(AttnArgs a) {
+  constexpr int NC = HD / 16;                 // channel tiles
+  constexpr int NK = HD / 32;                 // contraction steps of the scores
+  constexpr int LDO = HD + 4;
+  __shared__ float sm_o[NW][16][LDO];
+  __shared__ float sm_ml[NW][16][2];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r = lane & 15, g = lane >> 4;
+  const int split = blockIdx.x % a.splits, rt = blockIdx.x / a.splits;
+  const int h = blockIdx.y, s = blockIdx.z;
+  Span sp;
+  if (!span_of(a, s, rt * NQ * 16, rt * NQ * 16 + NQ * 16, sp)) return;
+  const int per = (sp.nt + a.splits - 1) / a.splits;
+  const int i_end = min(sp.nt, (split + 1) * per);
+  const long head = (long)s * a.H + h;
+  const uint8_t* kb = a.k8 + head * a.cap * HD;
+  const uint8_t* vb = a.v8 + head * a.cap * HD;
+  const float* ksb = a.ks + head * (a.cap >> a.bshift);
+  const float* vsb = a.vs + head * (a.cap >> a.bshift);
+
+  // queries: contraction slot (step, g, j) is channel 16 (4 (step / 2) + g) + 8 (step % 2) + j, for hd = 32 channel 8 g + j
+  bf16x8_v qf[NQ][NK];
+  int prow[NQ];                               // position of the lane's row
+#pragma unroll
+  for (int iq = 0; iq < NQ; ++iq) {
+    const int row = min(rt * NQ * 16 + iq * 16 + r, sp.rows - 1);
+    const int t = row / a.G, gq = row - t * a.G;
+    prow[iq] = sp.p0 + t;
+    const bf16_t* qp = a.q + a.q_ss * s + a.q_st * t + (long)(h * a.G + gq) * HD;
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+      const int ch = HD == 32 ? 8 * g : 16 * (4 * (k >> 1) + g) + 8 * (k & 1);
+      qf[iq][k] = *reinterpret_cast<const bf16x8_v*>(qp + ch);
+    }
+  }
+  f32x4 o[NQ][NC];
+  float m[NQ], l[NQ];
+#pragma unroll
+  for (int iq = 0; iq < NQ; ++iq) {
+    m[iq] = -INFINITY;
+    l[iq] = 0.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) o[iq][c] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  }
+  constexpr int KW = HD == 32 ? 2 : HD / 16;  // dwords of K per lane and 16-key row tile (8 B | 16 B | 32 B)
+  uint32_t kc[4][KW], kn[4][KW];
+  uint4 vc[NC], vn[NC];
+  float ksc = 0.f, vsc = 0.f, ksn = 0.f, vsn = 0.f;
+  auto load = [&](int tile, uint32_t (&kk)[4][KW], uint4 (&vv)[NC], float& kscale, float& vscale) {
+    const uint8_t* kp = kb + ((long)tile * KT + (r >> 2) * 16 + (r & 3)) * HD;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      if constexpr (HD == 32) {
+        const uint2 w = *reinterpret_cast<const uint2*>(kp + t * 4 * HD + g * 8);
+        kk[t][0] = w.x; kk[t][1] = w.y;
+      } else {
+#pragma unroll
+        for (int j = 0; j < HD / 64; ++j) {
+          const uint4 w = *reinterpret_cast<const uint4*>(kp + t * 4 * HD + (j * 4 + g) * 16);
+          kk[t][4 * j] = w.x; kk[t][4 * j + 1] = w.y; kk[t][4 * j + 2] = w.z; kk[t][4 * j + 3] = w.w;
+        }
+      }
+    }
+    const uint8_t* vp = vb + ((long)tile * 4 + g) * (HD * 16) + r * 16;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) vv[c] = *reinterpret_cast<const uint4*>(vp + c * 256);
+    const int b = (tile * KT + g * 16) >> a.bshift;
+    kscale = ksb[b];
+    vscale = vsb[b];
+  };
+  int it = split * per + wave;
+  if (it < i_end) load(tile_of(sp, it), kc, vc, ksc, vsc);
+  for (; it < i_end; it += NW) {
+    const int tile = tile_of(sp, it);
+    if (it + NW < i_end) load(tile_of(sp, it + NW), kn, vn, ksn, vsn);
+    const int key0 = tile * KT + g * 16;      // the lane's 16 positions
+    const bool plain = tile * KT >= sp.first && tile * KT + KT - 1 <= sp.pfirst && (a.window == 0 || tile * KT > sp.plast - a.window);
+    if (!plain) {                             // positions outside [first, plast] hold whatever was left there: out of V before it is multiplied by 0
+      const int lo = sp.first - key0, hi = sp.plast - key0;
+      uint32_t bm[4];
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        bm[d] = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (4 * d + e >= lo && 4 * d + e <= hi) bm[d] |= 0xffu << (8 * e);
+      }
+#pragma unroll
+      for (int c = 0; c < NC; ++c) { vc[c].x &= bm[0]; vc[c].y &= bm[1]; vc[c].z &= bm[2]; vc[c].w &= bm[3]; }
+      if (lo > 15 || hi < 0) { vsc = 0.f; ksc = 0.f; }
+    }
+    const float sc = ksc * a.scale_log2e;
+    bf16x8_v pf[NQ][2], pl[NQ][2];
+    f32x4 st[NQ][4];
+#pragma unroll
+    for (int iq = 0; iq < NQ; ++iq)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) st[iq][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int k = 0; k < NK; ++k) {
+        const bf16x8_v kf = kv8_frag<DT>(kc[t][2 * k], kc[t][2 * k + 1]);
+#pragma unroll
+        for (int iq = 0; iq < NQ; ++iq) st[iq][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[iq][k], st[iq][t], 0, 0, 0);
+      }
+#pragma unroll
+    for (int iq = 0; iq < NQ; ++iq) {
+      float x[16];
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[4 * t + i] = st[iq][t][i] * sc;
+          if (!plain) x[4 * t + i] = visible(a, sp, key0 + 4 * t + i, prow[iq]) ? x[4 * t + i] : -INFINITY;
+        }
+      float mx = x[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float mn = fmaxf(m[iq], mx);
+      const float ms = mn == -INFINITY ? 0.f : mn;
+      const float alpha = __builtin_amdgcn_exp2f(m[iq] - ms);
+      m[iq] = mn;
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        x[i] = __builtin_amdgcn_exp2f(x[i] - ms);
+        sum += x[i];
+        x[i] *= vsc;
+      }
+      l[iq] = l[iq] * alpha + sum;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) o[iq][c] *= alpha;
+      // the probabilities enter the product as two bf16 (value and remainder, 16 bits together): the loop waits for memory, and a single
+      // rounding would add as much again to the error as the output's own
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float y[8], z[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = x[8 * u + e];
+        pf[iq][u] = pack8_bf16(y);
+        const uint4 w = __builtin_bit_cast(uint4, pf[iq][u]);
+        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          z[2 * e] = y[2 * e] - __uint_as_float(ww[e] << 16);
+          z[2 * e + 1] = y[2 * e + 1] - __uint_as_float(ww[e] & 0xffff0000u);
+        }
+        pl[iq][u] = pack8_bf16(z);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const bf16x8_v v0 = kv8_frag<DT>(vc[c].x, vc[c].y), v1 = kv8_frag<DT>(vc[c].z, vc[c].w);
+#pragma unroll
+      for (int iq = 0; iq < NQ; ++iq) {
+        o[iq][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, pf[iq][0], o[iq][c], 0, 0, 0);
+        o[iq][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, pf[iq][1], o[iq][c], 0, 0, 0);
+        o[iq][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, pl[iq][0], o[iq][c], 0, 0, 0);
+        o[iq][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, pl[iq][1], o[iq][c], 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int w = 0; w < KW; ++w) kc[t][w] = kn[t][w];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) vc[c] = vn[c];
+    ksc = ksn;
+    vsc = vsn;
+  }
+
+  // the waves meet
+#pragma unroll
+  for (int iq = 0; iq < NQ; ++iq) {
+    l[iq] += __shfl_xor(l[iq], 16, 64);
+    l[iq] += __shfl_xor(l[iq], 32, 64);
+    if (iq) __syncthreads();
+#pragma unroll
+    for (int c = 0; c < NC; ++c) *reinterpret_cast<f32x4*>(&sm_o[wave][r][c * 16 + g * 4]) = o[iq][c];
+    if (g == 0) { sm_ml[wave][r][0] = m[iq]; sm_ml[wave][r][1] = l[iq]; }
+    __syncthreads();
+    for (int e = threadIdx.x; e < 16 * (HD / 4); e += NW * 64) {
+      const int row16 = e / (HD / 4), c4 = (e % (HD / 4)) * 4;
+      const int row = rt * NQ * 16 + iq * 16 + row16;
+      if (row >= sp.rows) continue;
+      float mm = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) mm = fmaxf(mm, sm_ml[w][row16][0]);
+      const float ms = mm == -INFINITY ? 0.f : mm;
+      float ll = 0.f;
+      f32x4 acc = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float f = __builtin_amdgcn_exp2f(sm_ml[w][row16][0] - ms);
+        ll = fmaf(f, sm_ml[w][row16][1], ll);
+        acc += *reinterpret_cast<const f32x4*>(&sm_o[w][row16][c4]) * f;
+      }
+      if (a.splits == 1) {
+        const float inv = ll == 0.f ? 0.f : 1.0f / ll;
+        const int t = row / a.G, gq = row - t * a.G;
+        uint2 pk;
+        pk.x = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+        pk.y = pack_bf16x2(acc[2] * inv, acc[3] * inv);
+        *reinterpret_cast<uint2*>(a.out + a.o_ss * s + a.o_st * t + (long)(h * a.G + gq) * HD + c4) = pk;
+      } else {
+        const long pr = (head * a.splits + split) * ((long)a.rtiles * NQ * 16) + row;
+        *reinterpret_cast<f32x4*>(a.part_o + pr * HD + c4) = acc;
+        if (c4 == 0) { a.part_ml[2 * pr] = mm; a.part_ml[2 * pr + 1] = ll; }
+      }
+    }
+  }
+}
+
+// the splits meet: HD / 4 lanes per row
+template <int HD>
+__global__ __launch_bounds__(256) void attn_kv8_merge_kernel(AttnArgs a, int rows_pad) {
+  constexpr int LR = HD / 4;
+  const int h = blockIdx.y, s = blockIdx.z;
+  const int row = blockIdx.x * (256 / LR) + threadIdx.x / LR;
+  const int c4 = (threadIdx.x % LR) * 4;
+  const int p = a.pos[s];
+  int n = min(a.n_new ? a.n_new[s] : a.T, a.T);
+  if (p < 0 || p >= a.cap || n <= 0) return;
+  n = min(n, a.cap - p);
+  if (row >= n * a.G) return;
+  const long base = ((long)s * a.H + h) * a.splits * rows_pad + row;
+  float mm = -INFINITY;
+  for (int i = 0; i < a.splits; ++i) mm = fmaxf(mm, a.part_ml[2 * (base + (long)i * rows_pad)]);
+  const float ms = mm == -INFINITY ? 0.f : mm;
+  float ll = 0.f;
+  f32x4 acc = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int i = 0; i < a.splits; ++i) {
+    const long pr = base + (long)i * rows_pad;
+    const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * pr] - ms);
+    ll = fmaf(f, a.part_ml[2 * pr + 1], ll);
+    acc += *reinterpret_cast<const f32x4*>(a.part_o + pr * HD + c4) * f;
+  }
+  const float inv = ll == 0.f ? 0.f : 1.0f / ll;
+  const int t = row / a.G, gq = row - t * a.G;
+  uint2 pk;
+  pk.x = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+  pk.y = pack_bf16x2(acc[2] * inv, acc[3] * inv);
+  *reinterpret_cast<uint2*>(a.out + a.o_ss * s + a.o_st * t + (long)(h * a.G + gq) * HD + c4) = pk;
+}
+
+struct Plan { int nq, nw, rtiles, splits; };
+Plan plan_of(int S, int H, int hd, int rows, int max_len) {
+  Plan p;
+  p.nq = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  if (p.nq == 4 && hd == 128) p.nq = 2;
+  p.nw = p.nq == 1 ? 8 : 4;
+  p.rtiles = (rows + p.nq * 16 - 1) / (p.nq * 16);
+  const long base = (long)S * H * p.rtiles;
+  const long tiles = (max_len + KT - 1) / KT;
+  long sp = (1024 + base - 1) / base;                  // workgroups wanted
+  const long most = (tiles + p.nw - 1) / p.nw;         // a tile per wave
+  p.splits = (int)(sp < 1 ? 1 : sp < most ? sp : most);
+  if (p.splits < 1) p.splits = 1;
+  return p;
+}
+
+template <int HD, int DT>
+int launch_rows(const AttnArgs& a, const Plan& p, hipStream_t s) {
+  const dim3 grid((unsigned)(p.splits * p.rtiles), a.H, a.S);
+  if (p.nq == 1) hipLaunchKernelGGL((attn_kv8_rows_kernel<HD, DT, 1, 8>), grid, dim3(512), 0, s, a);
+  else if (p.nq == 2) hipLaunchKernelGGL((attn_kv8_rows_kernel<HD, DT, 2, 4>), grid, dim3(256), 0, s, a);
+  else if constexpr (HD < 128) hipLaunchKernelGGL((attn_kv8_rows_kernel<HD, DT, 4, 4>), grid, dim3(256), 0, s, a);
+  NEKO_CHECK_LAUNCH();
+  if (p.splits > 1) {
+    const int rows = a.T * a.G, per = 256 / (HD / 4);
+    hipLaunchKernelGGL((attn_kv8_merge_kernel<HD>), dim3((rows + per - 1) / per, a.H, a.S), dim3(256), 0, s, a, p.rtiles * p.nq * 16);
+    NEKO_CHECK_LAUNCH();
+  }
+  return NEKO_OK;
+}
+
+}  // namespace
+
+long neko_attn_kv8_ws_floats_impl(int S, int H, int G, int cap, int hd, int T, int max_len) {
+  if (S <= 0 || H <= 0 || G <= 0 || T <= 0 || cap <= 0 || hd <= 0) return 0;
+  const Plan p = plan_of(S, H, hd, T * G, max_len > 0 && max_len < cap ? max_len : cap);
+  return p.splits > 1 ? (long)S * H * p.splits * p.rtiles * p.nq * 16 * (hd + 2) : 0;
+}
+
+int neko_attn_kv8_impl(const uint8_t* k8, const uint8_t* v8, const float* ks, const float* vs, int dtype, int S, int H, int cap, int hd, int block,
+                       const bf16_t* q, long q_ss, long q_st, bf16_t* out, long o_ss, long o_st, int G, int T, const int* pos, const int* n_new,
+                       const int* start, int window, int sinks, float scale, int max_len, float* ws, long ws_floats, hipStream_t s) {
+  if (!k8 || !v8 || !ks || !vs || !q || !out || !pos || G <= 0 || T <= 0 || window < 0 || sinks < 0) return NEKO_ERR_ARG;
+  const int rc = neko_kv8_geometry(dtype, S, H, cap, hd, block);
+  if (rc) return rc;
+  if (T > cap || (long)T * G > (1 << 24)) return NEKO_ERR_ARG;
+  if (((uintptr_t)q | (uintptr_t)out) & 15 || (q_ss | q_st | o_ss | o_st) & 7) return NEKO_ERR_ARG;
+  if (max_len <= 0 || max_len > cap) max_len = cap;
+  const Plan p = plan_of(S, H, hd, T * G, max_len);
+  const long need = neko_attn_kv8_ws_floats_impl(S, H, G, cap, hd, T, max_len);
+  if (need > ws_floats || (need && !ws)) return NEKO_ERR_ARG;
+  const int bshift = block == 16 ? 4 : block == 32 ? 5 : 6;
+  AttnArgs a{k8, v8, ks, vs, q, out, q_ss, q_st, o_ss, o_st, pos, n_new, start, ws, nullptr, S, H, G, cap, T, bshift, window, sinks, p.splits, p.rtiles,
+             scale * 1.4426950408889634f};
+  a.part_ml = ws + (long)S * H * p.splits * p.rtiles * p.nq * 16 * hd;
+#define NEKO_KV8_ATTN(HD) return dtype == 0 ? launch_rows<HD, 0>(a, p, s) : launch_rows<HD, 1>(a, p, s)
+  if (hd == 32) NEKO_KV8_ATTN(32);
+  if (hd == 64) NEKO_KV8_ATTN(64);
+  NEKO_KV8_ATTN(128);
+#undef NEKO_KV8_ATTN
+}

@@ -265,4 +265,35 @@ int neko_pack_embed_bwd_det(const int* desc, const long long* tokens, const floa
                                       S(stream));
 }
 
+int neko_kv8_append(void* k8, void* v8, float* k_scale, float* v_scale, int dtype, int nseq, int H, int cap, int hd, int block, const uint16_t* k,
+                    long k_ss, long k_st, const uint16_t* v, long v_ss, long v_st, const int* pos, const int* n_new, int T, void* stream) {
+  return neko_kv8_append_impl(static_cast<uint8_t*>(k8), static_cast<uint8_t*>(v8), k_scale, v_scale, dtype, nseq, H, cap, hd, block, k, k_ss, k_st,
+                              v, v_ss, v_st, pos, n_new, T, S(stream));
+}
+int neko_kv8_read(const void* k8, const void* v8, const float* k_scale, const float* v_scale, int dtype, int nseq, int H, int cap, int hd, int block,
+                  const int* length, int L, uint16_t* k, uint16_t* v, void* stream) {
+  return neko_kv8_read_impl(static_cast<const uint8_t*>(k8), static_cast<const uint8_t*>(v8), k_scale, v_scale, dtype, nseq, H, cap, hd, block, length,
+                            L, k, v, S(stream));
+}
+long neko_attn_kv8_ws_floats(int nseq, int H, int G, int cap, int hd, int T, int max_len) {
+  return neko_attn_kv8_ws_floats_impl(nseq, H, G, cap, hd, T, max_len);
+}
+int neko_attn_kv8(const void* k8, const void* v8, const float* k_scale, const float* v_scale, int dtype, int nseq, int H, int cap, int hd, int block,
+                  const uint16_t* q, long q_ss, long q_st, uint16_t* out, long o_ss, long o_st, int G, int T, const int* pos, const int* n_new,
+                  const int* start, int window, int sinks, float scale, int max_len, float* ws, long ws_floats, void* stream) {
+  return neko_attn_kv8_impl(static_cast<const uint8_t*>(k8), static_cast<const uint8_t*>(v8), k_scale, v_scale, dtype, nseq, H, cap, hd, block, q, q_ss,
+                            q_st, out, o_ss, o_st, G, T, pos, n_new, start, window, sinks, scale, max_len, ws, ws_floats, S(stream));
+}
+long neko_verify_draft_ws_bytes(int B, int K, int V) { return neko_verify_draft_ws_bytes_impl(B, K, V); }
+int neko_verify_draft(const void* target, long t_sb, long t_sr, const void* draft, long d_sb, long d_sr, int is_bf16, int B, int K, int V,
+                      const long long* tokens, const float* u, const float* r, const int* n_draft, float temperature, int* accepted,
+                      long long* out_tokens, void* ws, long ws_bytes, void* stream) {
+  return neko_verify_draft_impl(target, t_sb, t_sr, draft, d_sb, d_sr, is_bf16, B, K, V, tokens, u, r, n_draft, temperature, accepted, out_tokens,
+                                ws, ws_bytes, S(stream));
+}
+int neko_distill_topk(const void* z, long ldz, int is_bf16, int R, int V, int Vpad, const float* t_val, const int* t_idx, int k, const float* weight,
+                      float tau, const long long* target, float hard, float* loss_row, void* dlogits, long ldd, void* stream) {
+  return neko_distill_topk_impl(z, ldz, is_bf16, R, V, Vpad, t_val, t_idx, k, weight, tau, target, hard, loss_row, dlogits, ldd, S(stream));
+}
+
 }  // extern "C"

@@ -155,3 +155,19 @@ int neko_patch_pos_add_bwd_det_impl(const float* dout, const int* hpos, const in
                                     int d, int nrows, void* ws, long ws_bytes, hipStream_t s);
 int neko_patch_pos_add_bwd_impl(const float* dout, const int* hpos, const int* wpos, float* d_row_emb,
                                 float* d_col_emb, int P, int d, hipStream_t s);
+// 8-bit key / value cache (kv8.h, kv8.hip, attention_kv8.hip): dtype 0 = e4m3, 1 = int8
+int neko_kv8_geometry(int dtype, int S, int H, int cap, int hd, int block);
+int neko_kv8_append_impl(uint8_t* k8, uint8_t* v8, float* ks, float* vs, int dtype, int S, int H, int cap, int hd, int block, const bf16_t* k, long k_ss,
+                         long k_st, const bf16_t* v, long v_ss, long v_st, const int* pos, const int* n_new, int T, hipStream_t s);
+int neko_kv8_read_impl(const uint8_t* k8, const uint8_t* v8, const float* ks, const float* vs, int dtype, int S, int H, int cap, int hd, int block,
+                       const int* length, int L, bf16_t* k, bf16_t* v, hipStream_t s);
+long neko_attn_kv8_ws_floats_impl(int S, int H, int G, int cap, int hd, int T, int max_len);
+int neko_attn_kv8_impl(const uint8_t* k8, const uint8_t* v8, const float* ks, const float* vs, int dtype, int S, int H, int cap, int hd, int block,
+                       const bf16_t* q, long q_ss, long q_st, bf16_t* out, long o_ss, long o_st, int G, int T, const int* pos, const int* n_new,
+                       const int* start, int window, int sinks, float scale, int max_len, float* ws, long ws_floats, hipStream_t s);
+long neko_verify_draft_ws_bytes_impl(int B, int K, int V);
+int neko_verify_draft_impl(const void* target, long t_sb, long t_sr, const void* draft, long d_sb, long d_sr, int is_bf16, int B, int K, int V,
+                           const long long* tokens, const float* u, const float* r, const int* n_draft, float temperature, int* accepted,
+                           long long* out, void* ws, long ws_bytes, hipStream_t s);
+int neko_distill_topk_impl(const void* z, long ldz, int is_bf16, int R, int V, int Vpad, const float* t_val, const int* t_idx, int k, const float* weight,
+                           float tau, const long long* target, float hard, float* loss_row, void* dlogits, long ldd, hipStream_t s);

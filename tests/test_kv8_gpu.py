@@ -1,0 +1,272 @@
+"""The 8-bit key / value cache and the attention over it, through the tensor-level entry points, against 64-bit restatements."""
+import pytest
+import torch
+
+from serving_ref import RefCache, attention
+
+pytestmark = pytest.mark.gpu
+E4, I8 = torch.float8_e4m3fn, torch.int8
+BF16 = torch.bfloat16
+
+
+def _rows(S, T, H, hd, g, spread=1.0):
+    """K and V as views of one fused [S, T, 3, H, hd] projection."""
+    x = torch.randn(S, T, 3, H, hd, generator=g) * torch.exp(spread * torch.randn(S, T, 3, H, 1, generator=g))
+    return x.to(BF16)
+
+
+def _dev_i(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def _check_cache(cache, ref, length):
+    from neko_amd import ops
+    k, v = ops.kv8_read(cache, _dev_i(length), cache.cap)
+    rk, rv = ref.read(length, cache.cap)
+    assert torch.equal(k.cpu().double(), rk) and torch.equal(v.cpu().double(), rv)
+    for got, want, n in ((cache.k_scale, ref.scale[0], length), (cache.v_scale, ref.scale[1], length)):
+        for s in range(cache.nseq):
+            nb = (n[s] + cache.block - 1) // cache.block
+            assert torch.equal(got[s, :, :nb].cpu().double(), want[s, :, :nb])
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("block", [16, 32, 64])
+@pytest.mark.parametrize("dtype", [E4, I8], ids=["e4m3", "int8"])
+def test_append_read_bitexact(hd, block, dtype):
+    """Several appends of different lengths, at positions inside a block, with growing magnitudes (older codes are rounded again)."""
+    from neko_amd import ops
+    S, H, cap = 3, 5, 192
+    g = torch.Generator().manual_seed(hd + block)
+    cache = ops.KV8Cache(S, H, cap, hd, dtype=dtype, block=block)
+    ref = RefCache(S, H, cap, hd, dtype, block)
+    pos = [0, 7, 100]
+    ref_pos0 = list(pos)
+    # positions below the first append were written earlier
+    x = _rows(S, 100, H, hd, g)
+    ops.kv8_append(cache, x.cuda()[:, :, 1], x.cuda()[:, :, 2], _dev_i([0, 0, 0]), n_new=_dev_i(ref_pos0))
+    ref.append(x[:, :, 1], x[:, :, 2], [0, 0, 0], ref_pos0)
+    for T, n in ((1, [1, 1, 1]), (5, [5, 0, 3]), (40, [40, 33, 17]), (1, [1, 1, 1]), (64, [64, 64, 64])):
+        x = _rows(S, T, H, hd, g) * (1.0 + T)
+        xd = x.cuda()
+        ops.kv8_append(cache, xd[:, :, 1], xd[:, :, 2], _dev_i(pos), n_new=_dev_i(n))
+        ref.append(x[:, :, 1], x[:, :, 2], pos, n)
+        pos = [min(cap, p + m) for p, m in zip(pos, n)]
+        _check_cache(cache, ref, pos)
+
+
+@pytest.mark.parametrize("dtype", [E4, I8], ids=["e4m3", "int8"])
+def test_append_edges(dtype):
+    """Past the end, outside, zero rows, NaN and infinities, a block that starts afresh, bytes behind the new rows untouched."""
+    from neko_amd import ops
+    S, H, cap, hd, block = 6, 2, 64, 32, 32
+    g = torch.Generator().manual_seed(1)
+    cache = ops.KV8Cache(S, H, cap, hd, dtype=dtype, block=block)
+    cache.k.view(torch.uint8).fill_(0x35)
+    cache.v.view(torch.uint8).fill_(0x35)
+    before_k, before_v = cache.k.view(torch.uint8).clone(), cache.v.view(torch.uint8).clone()
+    x = _rows(S, 9, H, hd, g)
+    x[0, 0, 1:, 0, :4] = torch.tensor([float("nan"), float("inf"), -float("inf"), 1.0])
+    x[1] = 0
+    pos, n = [0, 0, 60, 64, -3, 5], [9, 9, 9, 9, 9, 0]
+    xd = x.cuda()
+    ops.kv8_append(cache, xd[:, :, 1], xd[:, :, 2], _dev_i(pos), n_new=_dev_i(n))
+    ref = RefCache(S, H, cap, hd, dtype, block)
+    ref.codes = [torch.full_like(c, 0) for c in ref.codes]
+    ref.append(x[:, :, 1], x[:, :, 2], pos, n)
+    k, v = ops.kv8_read(cache, _dev_i([9, 9, 64, 0, 0, 0]), cap)
+    rk, rv = ref.read([9, 9, 64, 0, 0, 0], cap)
+    assert torch.equal(k[0].cpu().double(), rk[0]) and torch.equal(v[0].cpu().double(), rv[0])
+    assert torch.equal(k[1].cpu().double(), rk[1]) and torch.equal(v[1].cpu().double(), rv[1])
+    assert torch.equal(k[2, 60:].cpu().double(), rk[2, 60:]) and torch.equal(v[2, 60:].cpu().double(), rv[2, 60:])
+    assert int(k[3:].count_nonzero()) == 0
+    ku, vu = cache.k.view(torch.uint8), cache.v.view(torch.uint8)
+    assert torch.equal(ku[:, :, 9:60], before_k[:, :, 9:60]) and torch.equal(ku[3:], before_k[3:])
+    rows = vu.transpose(3, 4).reshape(S, H, cap, hd)
+    rows0 = before_v.transpose(3, 4).reshape(S, H, cap, hd)
+    assert torch.equal(rows[:2, :, 9:], rows0[:2, :, 9:]) and torch.equal(rows[3:], rows0[3:])
+    # set back to 0 and written again: the block forgets its scale
+    y = torch.full((S, 1, 3, H, hd), 2.0 ** -20, dtype=BF16)
+    yd = y.cuda()
+    ops.kv8_append(cache, yd[:, :, 1], yd[:, :, 2], _dev_i([0] * S))
+    assert float(cache.k_scale[0, 0, 0]) < 2.0 ** -20
+    k, _ = ops.kv8_read(cache, _dev_i([1] * S), 1)
+    assert torch.equal(k, yd[:, :, 1])
+
+
+def _attn_case(S, H, G, hd, cap, T, pos, n, start, window, sinks, dtype, block, seed=0, poison=True):
+    from neko_amd import ops
+    g = torch.Generator().manual_seed(seed)
+    ref = RefCache(S, H, cap, hd, dtype, block)
+    end = [max(0, min(cap, p + min(m, T))) if 0 <= p < cap else 0 for p, m in zip(pos, n)]
+    x = _rows(S, cap, H, hd, g, spread=0.4)
+    ref.append(x[:, :, 1], x[:, :, 2], [0] * S, end)
+    cache = ops.KV8Cache(S, H, cap, hd, dtype=dtype, block=block)
+    if poison:      # whatever lies outside [start, last row] must not matter: NaN codes (e4m3) or large ones, wild scales
+        cache.k.view(torch.uint8).fill_(0x7f)
+        cache.v.view(torch.uint8).fill_(0x7f)
+        cache.k_scale.fill_(float("inf"))
+        cache.v_scale.fill_(float("nan"))
+    xd = x.cuda()
+    ops.kv8_append(cache, xd[:, :, 1], xd[:, :, 2], _dev_i([0] * S), n_new=_dev_i(end))
+    if poison:      # positions before start: NaN values under a finite scale
+        ku, vu = cache.k.view(torch.uint8), cache.v.view(torch.uint8)
+        for s in range(S):
+            if start[s] > 0:
+                ku[s, :, :start[s]] = 0x7f
+                full = start[s] // 16
+                vu[s, :, :full] = 0x7f
+                if start[s] % 16:
+                    vu[s, :, full, :, :start[s] % 16] = 0x7f
+    q = torch.randn(S, T, H * G, hd, generator=g).to(BF16)
+    out0 = torch.full((S, T, H * G, hd), 7.0, dtype=BF16)
+    out = out0.cuda()
+    ops.attn_kv8(cache, q.cuda(), _dev_i(pos), n_new=_dev_i(n), start=_dev_i(start), window=window, sinks=sinks, out=out)
+    want, absv, big = attention(q, ref.values(0), ref.values(1), pos, n, start, window, sinks, hd ** -0.5, out0)
+    # output rounding 2^-8 |o|; probabilities: rounded to bf16 (2^-8, more than 64 rows a key head) or kept to 16 bits (2^-16); a score's
+    # fp32 sum of hd products of magnitude `big` in any order, in numerator and normaliser; sums of up to cap terms; exponential 2^-21
+    p_round = 2.0 ** -8 if T * G > 64 else 2.0 ** -16
+    tol = 2.0 ** -8 * want.abs() + (p_round + 2 * hd * 2.0 ** -23 * big + cap * 2.0 ** -23 + 2.0 ** -21) * absv
+    err = (out.cpu().double() - want).abs()
+    assert bool((err <= tol).all()), float((err - tol).max())
+    for s in range(S):      # rows behind a sequence's last
+        last = min(n[s], T, cap - pos[s]) if 0 <= pos[s] < cap else 0
+        assert torch.equal(out[s, max(0, last):].cpu(), out0[s, max(0, last):])
+
+
+@pytest.mark.parametrize("dtype", [E4, I8], ids=["e4m3", "int8"])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("T,G", [(1, 1), (1, 4), (6, 3), (7, 8), (70, 1), (40, 3)])
+def test_attn_rows(T, G, hd, dtype):
+    """One row, a few, more than one row tile; grouped heads; lengths of one position, of tile borders, at the end of the cache."""
+    cap = 320
+    pos = [0, 63 - min(T, 63), 64, 129, cap - T, 200]
+    n = [T] * 5 + [max(1, T // 2)]
+    _attn_case(6, 2, G, hd, cap, T, pos, n, [0] * 6, 0, 0, dtype, {32: 16, 64: 32, 128: 64}[hd], seed=T + hd)
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (17, 0), (64, 4), (100, 70), (500, 3)])
+@pytest.mark.parametrize("T", [1, 5, 80])
+def test_attn_window_start_empty(T, window, sinks):
+    """Windows and sinks around tile borders, left padding, rows that see nothing, sequences without rows."""
+    cap = 256
+    pos = [0, 100, cap - T, 30, 50, -1, cap, 150]
+    n = [T, T, T, T, 0, T, T, 1]
+    start = [0, 37, 64, 33 + T // 2, 0, 0, 0, 149]
+    _attn_case(8, 2, 2, 64, cap, T, pos, n, start, window, sinks, E4, 16, seed=window)
+
+
+def test_attn_all_before_start():
+    _attn_case(2, 1, 1, 32, 64, 3, [0, 10], [3, 3], [40, 5], 0, 0, I8, 32)
+
+
+def test_attn_strides_and_heads():
+    """q inside a fused projection, out inside a wider buffer; default output and counts."""
+    from neko_amd import ops
+    S, H, hd, T, cap = 2, 3, 64, 4, 128
+    g = torch.Generator().manual_seed(5)
+    x = _rows(S, T, H, hd, g)
+    xd = x.cuda()
+    cache = ops.KV8Cache(S, H, cap, hd, dtype=I8, block=64)
+    pos = _dev_i([0, 0])
+    ops.kv8_append(cache, xd[:, :, 1], xd[:, :, 2], pos)
+    a = ops.attn_kv8(cache, xd[:, :, 0], pos)
+    wide = torch.zeros(S, T, 2, H, hd, dtype=BF16, device="cuda")
+    b = ops.attn_kv8(cache, xd[:, :, 0].contiguous(), pos, out=wide[:, :, 1], max_len=T)
+    assert torch.equal(a, b) and torch.equal(wide[:, :, 1], a) and int(wide[:, :, 0].count_nonzero()) == 0
+    assert torch.equal(a[:, 0], ops.kv8_read(cache, _dev_i([1, 1]), 1)[1][:, 0])       # the first row sees itself only
+
+
+@pytest.mark.parametrize("max_len", [0, 64, 2048])
+def test_attn_splits_agree(max_len):
+    """The split of the key axis (sized by max_len) changes nothing but roundings; two calls of one split are bit-equal."""
+    from neko_amd import ops
+    S, H, hd, cap = 1, 2, 64, 2048
+    g = torch.Generator().manual_seed(9)
+    x = _rows(S, cap, H, hd, g, spread=0.3)
+    xd = x.cuda()
+    cache = ops.KV8Cache(S, H, cap, hd, block=32)
+    ops.kv8_append(cache, xd[:, :, 1], xd[:, :, 2], _dev_i([0]))
+    q = torch.randn(S, 1, H, hd, generator=g).to(BF16).cuda()
+    a = ops.attn_kv8(cache, q, _dev_i([cap - 1]), max_len=max_len)
+    assert torch.equal(a, ops.attn_kv8(cache, q, _dev_i([cap - 1]), max_len=max_len))
+    k, v = (t.cpu().double().transpose(1, 2) for t in ops.kv8_read(cache, _dev_i([cap]), cap))
+    want, absv, big = attention(q.cpu(), k, v, [cap - 1], [1], [0], 0, 0, hd ** -0.5, torch.zeros(S, 1, H, hd))
+    tol = 2.0 ** -8 * want.abs() + (2.0 ** -16 + 2 * hd * 2.0 ** -23 * big + cap * 2.0 ** -23 + 2.0 ** -21) * absv
+    assert bool(((a.cpu().double() - want).abs() <= tol).all())
+
+
+def test_large_offsets():
+    """A cache whose bytes pass 2^32: the last sequence's rows land where they belong, the first one's stay."""
+    from neko_amd import ops
+    S, H, hd, cap = 5, 16, 128, 1 << 19
+    k = torch.zeros(S, H, cap, hd, dtype=torch.uint8, device="cuda").view(I8)
+    v = torch.zeros(S, H, cap // 16, hd, 16, dtype=torch.uint8, device="cuda").view(I8)
+    ks = torch.ones(S, H, cap // 64, device="cuda")
+    vs = torch.ones_like(ks)
+    cache = ops.KV8Cache.from_tensors(k, v, ks, vs)
+    x = torch.randn(S, 2, 3, H, hd, device="cuda").to(BF16)
+    pos = _dev_i([0, 1, 2, 3, cap - 2])
+    ops.kv8_append(cache, x[:, :, 1], x[:, :, 2], pos)
+    start = pos.clone()
+    o = ops.attn_kv8(cache, x[:, :, 0], pos, start=start)
+    small = ops.KV8Cache(S, H, 64, hd, dtype=I8, block=64)
+    there = _dev_i([0, 1, 2, 3, 62])                             # the same places inside a block, older rows of zeros under a scale of 1
+    ops.kv8_append(small, x[:, :, 1], x[:, :, 2], there)
+    want = ops.attn_kv8(small, x[:, :, 0], there, start=there)
+    assert torch.equal(o[:, 0], want[:, 0])                      # one visible key: its value
+    assert float((o.float() - want.float()).abs().max()) <= 2.0 ** -7 * float(want.float().abs().max())
+
+
+def test_two_streams_and_capture():
+    """Append and attention captured into a graph that advances the positions; two graphs and eager calls in between."""
+    from neko_amd import ops
+    S, H, hd, cap, N = 2, 2, 32, 128, 12
+    g = torch.Generator().manual_seed(3)
+    x = _rows(S, N, H, hd, g).cuda()
+
+    def eager(dtype):
+        cache = ops.KV8Cache(S, H, cap, hd, dtype=dtype)
+        pos = _dev_i([0, 3])
+        outs = []
+        for i in range(N):
+            ops.kv8_append(cache, x[:, i:i + 1, 1], x[:, i:i + 1, 2], pos)
+            outs.append(ops.attn_kv8(cache, x[:, i:i + 1, 0], pos, start=_dev_i([0, 3])))
+            pos += 1
+        return torch.cat(outs, 1)
+
+    class Graph:
+        def __init__(self, dtype):
+            self.cache = ops.KV8Cache(S, H, cap, hd, dtype=dtype)
+            self.pos, self.start = _dev_i([0, 3]), _dev_i([0, 3])
+            self.row = torch.zeros(S, 1, 3, H, hd, dtype=BF16, device="cuda")
+            self.out = torch.zeros(S, 1, H, hd, dtype=BF16, device="cuda")
+            self.graph = torch.cuda.CUDAGraph()
+            torch.cuda.synchronize()
+            with torch.cuda.graph(self.graph):
+                ops.kv8_append(self.cache, self.row[:, :, 1], self.row[:, :, 2], self.pos)
+                ops.attn_kv8(self.cache, self.row[:, :, 0], self.pos, start=self.start, out=self.out)
+                self.pos.add_(1)
+
+        def step(self, r):
+            self.row.copy_(r)
+            self.graph.replay()
+            return self.out.clone()
+
+    want = {d: eager(d) for d in (E4, I8)}
+    graphs = {d: Graph(d) for d in (E4, I8)}
+    got = {E4: [], I8: []}
+    for i in range(N):
+        for d in (E4, I8):
+            got[d].append(graphs[d].step(x[:, i:i + 1]))
+        if i % 3 == 0:
+            assert torch.equal(eager(E4)[:, :i + 1], want[E4][:, :i + 1])
+            torch.cuda.synchronize()
+    for d in (E4, I8):
+        assert torch.equal(torch.cat(got[d], 1), want[d])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = eager(I8)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(other, want[I8])
