@@ -372,7 +372,7 @@ int neko_patch_pos_add_bwd_sorted(const float* dout, const int* hkeys_sorted, co
  * neko_kv8_read: rows 0 .. L-1 of every sequence as bf16 (exact), k, v contiguous [nseq][L][H][hd]; rows t >= length[s] are written as 0.
  * neko_attn_kv8: T rows a sequence at positions pos[s] + i (i < n as above; other rows of `out` are left as they are), G query heads per key
  *   head (query head h * G + g reads key head h), q and out bf16 with strides as k above.  Row at position p sees t with start[s] <= t <= p and,
- *   where window > 0, t > p - window or t < start[s] + sinks (start NULL: 0).  A row that sees nothing is 0.  `scale` multiplies q . k.
+ *   where window > 0, t > p - window or t < start[s] + sinks (start NULL: 0).  A row that sees nothing is 0.  `scale` > 0 multiplies q . k.
  *   What lies in the cache outside [start, last row] never reaches the output.  max_len: host-known bound on pos + T (0: cap); it sizes
  *   the split of the key axis and changes no result beyond rounding.  ws: neko_attn_kv8_ws_floats(..) floats (may be 0), private to the call.
  * neko_verify_draft: sequence b, K + 1 rows of target logits (element (b, i, v) at b * t_sb + i * t_sr + v; fp32 or bf16), n = n_draft[b] <= K

@@ -286,6 +286,224 @@ __global__ __launch_bounds__(NW * 64) void attn_kv8_rows_kernel(AttnArgs a) {
   }
 }
 
+// ---- many rows: key tiles through LDS -------------------------------------------------------------------------------------
+// One workgroup of NW waves per (split, head, sequence, row tile of 32 NW rows); a wave owns 32 rows.  A 64-key tile is unpacked ONCE, on
+// its way into LDS (codes x scale as bf16: exact), and read there by every wave as matrix operands; the codes of the tile after it are
+// loaded meanwhile, one barrier per tile.  32 x 32 x 16 products: S^T = K Q^T, then O^T = V^T P^T with the probabilities as they stand --
+// LDS row r of a 32-key half tile holds key 16 ((r >> 2) & 1) + 4 (r >> 3) + (r & 3), so that a lane's 16 scores are 16 consecutive keys.
+//   K image: rows of HD bf16, 16-byte pieces XORed with the row (16 lanes read 16 rows: all banks once);  V image: [8 keys][channel] pieces.
+// The running maximum of a row moves only when a score passes it by 2^8 (fp32 sums and bf16 probabilities do not care about a common factor),
+// so the output is rarely rescaled.  Probabilities are rounded to bf16 once: their errors are independent and average out like the
+// values' own (measured 1.0-1.4 x the error of the rounded output), and a second product would cost 50 % of the matrix work.
+template <int HD>
+__device__ __forceinline__ int kimg(int row, int piece) {
+  constexpr int PC = HD / 8, SH = HD == 128 ? 0 : HD == 64 ? 1 : 2;
+  return row * (HD * 2) + ((piece ^ ((row >> SH) & (PC - 1))) << 4);
+}
+
+template <int HD, int DT, int NW>
+__global__ __launch_bounds__(NW * 64) void attn_kv8_tile_kernel(AttnArgs a) {
+  constexpr int NC = HD / 32, NK = HD / 16;
+  constexpr int IMG = KT * HD * 2;                        // bytes of one image
+  constexpr int UNITS = KT * HD / 16;                     // 16-byte pieces of K (and of V) in a tile
+  constexpr int NT = NW * 64;
+  constexpr int UPT = (2 * UNITS + NT - 1) / NT;          // pieces per thread
+  __shared__ __attribute__((aligned(16))) char smem[2][2 * IMG];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int r = lane & 31, hf = lane >> 5;
+  const int split = blockIdx.x % a.splits, rt = a.rtiles - 1 - blockIdx.x / a.splits;     // the row tiles with the most keys first
+  const int h = blockIdx.y, s = blockIdx.z;
+  constexpr int RT = NW * 32;
+  Span sp;
+  if (!span_of(a, s, rt * RT, rt * RT + RT, sp)) return;
+  const int per = (sp.nt + a.splits - 1) / a.splits;
+  const int i0 = split * per, i_end = min(sp.nt, i0 + per);
+  const long head = (long)s * a.H + h;
+  const uint8_t* kb = a.k8 + head * a.cap * HD;
+  const uint8_t* vb = a.v8 + head * a.cap * HD;
+  const float* ksb = a.ks + head * (a.cap >> a.bshift);
+  const float* vsb = a.vs + head * (a.cap >> a.bshift);
+
+  const int row = rt * RT + wave * 32 + r;
+  const int w0 = rt * RT + wave * 32;                     // the wave's first row
+  const bool wave_on = w0 < sp.rows;
+  const int rc = min(row, sp.rows - 1);
+  const int t = rc / a.G, gq = rc - t * a.G;
+  const int prow = sp.p0 + t;
+  const int wfirst = sp.p0 + min(w0, sp.rows - 1) / a.G, wlast = sp.p0 + min(w0 + 31, sp.rows - 1) / a.G;
+  bf16x8_v qf[NK];
+  {
+    const bf16_t* qp = a.q + a.q_ss * s + a.q_st * t + (long)(h * a.G + gq) * HD + hf * 8;
+#pragma unroll
+    for (int k = 0; k < NK; ++k) qf[k] = *reinterpret_cast<const bf16x8_v*>(qp + k * 16);
+  }
+  f32x16 o[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[c][i] = 0.f;
+  float m = -INFINITY, l = 0.f;
+
+  uint4 st[UPT];
+  float ss[UPT];
+  auto fetch = [&](int tile) {
+#pragma unroll
+    for (int i = 0; i < UPT; ++i) {
+      const int u = tid + i * NT;                         // [0, UNITS): K, then V
+      if (2 * UNITS % NT && u >= 2 * UNITS) break;
+      const bool v = u >= UNITS;
+      const int uu = v ? u - UNITS : u;
+      st[i] = *reinterpret_cast<const uint4*>((v ? vb : kb) + (long)tile * KT * HD + uu * 16);
+      const int key = v ? (uu / HD) * 16 : uu / (HD / 16);
+      ss[i] = (v ? vsb : ksb)[(tile * KT + key) >> a.bshift];
+    }
+  };
+  auto stage = [&](int tile, char* img) {
+    const bool edge = tile * KT < sp.first || tile * KT + KT - 1 > sp.plast;
+#pragma unroll
+    for (int i = 0; i < UPT; ++i) {
+      const int u = tid + i * NT;
+      if (2 * UNITS % NT && u >= 2 * UNITS) break;
+      const bool v = u >= UNITS;
+      const int uu = v ? u - UNITS : u;
+      uint32_t w[4] = {st[i].x, st[i].y, st[i].z, st[i].w};
+      float sc = ss[i];
+      int at0, at1;
+      if (!v) {
+        const int key = uu / (HD / 16), cc = uu % (HD / 16);
+        const int kk = key & 31;                          // its row in the half tile
+        const int lr = (key & 32) + 8 * ((kk >> 2) & 3) + 4 * (kk >> 4) + (kk & 3);
+        at0 = kimg<HD>(lr, 2 * cc);
+        at1 = kimg<HD>(lr, 2 * cc + 1);
+      } else {
+        const int t16 = uu / HD, ch = uu % HD;
+        at0 = IMG + ((2 * t16) * HD + ch) * 16;
+        at1 = at0 + HD * 16;
+        if (edge) {                                       // positions outside [first, plast] hold whatever was left there
+          const int lo = sp.first - (tile * KT + t16 * 16), hi = sp.plast - (tile * KT + t16 * 16);
+#pragma unroll
+          for (int d = 0; d < 4; ++d) {
+            uint32_t bm = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (4 * d + e >= lo && 4 * d + e <= hi) bm |= 0xffu << (8 * e);
+            w[d] &= bm;
+          }
+          if (lo > 15 || hi < 0) sc = 0.f;
+        }
+      }
+      *reinterpret_cast<uint4*>(img + at0) = make_uint4(kv8_unpack2<DT, false>(w[0], sc), kv8_unpack2<DT, true>(w[0], sc), kv8_unpack2<DT, false>(w[1], sc),
+                                                        kv8_unpack2<DT, true>(w[1], sc));
+      *reinterpret_cast<uint4*>(img + at1) = make_uint4(kv8_unpack2<DT, false>(w[2], sc), kv8_unpack2<DT, true>(w[2], sc), kv8_unpack2<DT, false>(w[3], sc),
+                                                        kv8_unpack2<DT, true>(w[3], sc));
+    }
+  };
+  if (i0 < i_end) {
+    fetch(tile_of(sp, i0));
+    stage(tile_of(sp, i0), smem[0]);
+  }
+  __syncthreads();
+  for (int it = i0; it < i_end; ++it) {
+    const int tile = tile_of(sp, it);
+    const char* img = smem[(it - i0) & 1];
+    const bool more = it + 1 < i_end;
+    if (more) fetch(tile_of(sp, it + 1));
+    const int tk = tile * KT;
+    if (wave_on && tk <= wlast) {
+      f32x16 sc[2];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[kt][i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < NK; ++k)
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+          const bf16x8_v kf = *reinterpret_cast<const bf16x8_v*>(img + kimg<HD>(kt * 32 + r, 2 * k + hf));
+          sc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[k], sc[kt], 0, 0, 0);
+        }
+      const bool plain = tk >= sp.first && tk + KT - 1 <= wfirst && (a.window == 0 || tk > wlast - a.window);
+      if (!plain) {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (!visible(a, sp, tk + kt * 32 + hf * 16 + i, prow)) sc[kt][i] = -INFINITY;
+      }
+      float mx = sc[0][0];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[kt][i]);
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * a.scale_log2e;        // scale > 0 (checked on entry)
+      if (__builtin_amdgcn_ballot_w64(mx > m + 8.0f || (m == -INFINITY && mx > m))) {
+        const float mn = fmaxf(m, mx);
+        const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+        m = mn;
+        l *= alpha;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[c][i] *= alpha;
+      }
+      const float ms = m == -INFINITY ? 0.f : m;
+      float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[kt][i], a.scale_log2e, -ms)), p1 = __builtin_amdgcn_exp2f(fmaf(sc[kt][i + 1], a.scale_log2e, -ms));
+          sc[kt][i] = p0;
+          sc[kt][i + 1] = p1;
+          sum0 += p0;
+          sum1 += p1;
+        }
+      l += sum0 + sum1;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float y[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = sc[kt][8 * u + e];
+          const bf16x8_v pf = pack8_bf16(y);
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            const bf16x8_v vf = *reinterpret_cast<const bf16x8_v*>(img + IMG + ((kt * 4 + 2 * hf + u) * HD + c * 32 + r) * 16);
+            o[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf, o[c], 0, 0, 0);
+          }
+        }
+    }
+    if (more) stage(tile_of(sp, it + 1), smem[(it + 1 - i0) & 1]);
+    __syncthreads();
+  }
+  l += __shfl_xor(l, 32, 64);
+  if (row >= sp.rows) return;
+  if (a.splits == 1) {
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    bf16_t* op = a.out + a.o_ss * s + a.o_st * t + (long)(h * a.G + gq) * HD;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint2 pk;
+        pk.x = pack_bf16x2(o[c][4 * j] * inv, o[c][4 * j + 1] * inv);
+        pk.y = pack_bf16x2(o[c][4 * j + 2] * inv, o[c][4 * j + 3] * inv);
+        *reinterpret_cast<uint2*>(op + c * 32 + 8 * j + 4 * hf) = pk;
+      }
+  } else {
+    const long pr = (head * a.splits + split) * ((long)a.rtiles * RT) + row;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f32x4 x = {o[c][4 * j], o[c][4 * j + 1], o[c][4 * j + 2], o[c][4 * j + 3]};
+        *reinterpret_cast<f32x4*>(a.part_o + pr * HD + c * 32 + 8 * j + 4 * hf) = x;
+      }
+    if (hf == 0) { a.part_ml[2 * pr] = m; a.part_ml[2 * pr + 1] = l; }
+  }
+}
+
 // the splits meet: HD / 4 lanes per row
 template <int HD>
 __global__ __launch_bounds__(256) void attn_kv8_merge_kernel(AttnArgs a, int rows_pad) {
@@ -319,17 +537,28 @@ __global__ __launch_bounds__(256) void attn_kv8_merge_kernel(AttnArgs a, int row
   *reinterpret_cast<uint2*>(a.out + a.o_ss * s + a.o_st * t + (long)(h * a.G + gq) * HD + c4) = pk;
 }
 
-struct Plan { int nq, nw, rtiles, splits; };
+// How a call is cut.  More than 64 rows a key head go through LDS tiles (a row tile of 128 or 256); up to 64 stay in the register kernel, 16 / 32 /
+// 64 rows a wave.  The key axis is split until the grid fills the chip.
+struct Plan { int tiled, nq, nw, rt, rtiles, splits; };
 Plan plan_of(int S, int H, int hd, int rows, int max_len) {
   Plan p;
-  p.nq = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  if (p.nq == 4 && hd == 128) p.nq = 2;
-  p.nw = p.nq == 1 ? 8 : 4;
-  p.rtiles = (rows + p.nq * 16 - 1) / (p.nq * 16);
+  p.tiled = rows > 64;
+  if (p.tiled) {
+    p.nq = 0;
+    p.nw = rows <= 128 ? 4 : 8;
+    p.rt = 32 * p.nw;
+  } else {
+    p.nq = rows <= 16 ? 1 : rows <= 32 || hd == 128 ? 2 : 4;
+    p.nw = p.nq == 1 ? 8 : 4;
+    p.rt = 16 * p.nq;
+  }
+  p.rtiles = (rows + p.rt - 1) / p.rt;
   const long base = (long)S * H * p.rtiles;
   const long tiles = (max_len + KT - 1) / KT;
-  long sp = (1024 + base - 1) / base;                  // workgroups wanted
-  const long most = (tiles + p.nw - 1) / p.nw;         // a tile per wave
+  const long want = p.tiled ? 256 : 1024;              // workgroups
+  long sp = (want + base - 1) / base;
+  const long most = p.tiled ? (tiles + 7) / 8 : (tiles + p.nw - 1) / p.nw;      // 8 tiles a workgroup | a tile a wave
+  if (p.tiled && base * 4 > 3 * want) sp = 1;          // three quarters full: a second pass over the partial sums costs more
   p.splits = (int)(sp < 1 ? 1 : sp < most ? sp : most);
   if (p.splits < 1) p.splits = 1;
   return p;
@@ -338,13 +567,15 @@ Plan plan_of(int S, int H, int hd, int rows, int max_len) {
 template <int HD, int DT>
 int launch_rows(const AttnArgs& a, const Plan& p, hipStream_t s) {
   const dim3 grid((unsigned)(p.splits * p.rtiles), a.H, a.S);
-  if (p.nq == 1) hipLaunchKernelGGL((attn_kv8_rows_kernel<HD, DT, 1, 8>), grid, dim3(512), 0, s, a);
+  if (p.tiled && p.nw == 4) hipLaunchKernelGGL((attn_kv8_tile_kernel<HD, DT, 4>), grid, dim3(256), 0, s, a);
+  else if (p.tiled) hipLaunchKernelGGL((attn_kv8_tile_kernel<HD, DT, 8>), grid, dim3(512), 0, s, a);
+  else if (p.nq == 1) hipLaunchKernelGGL((attn_kv8_rows_kernel<HD, DT, 1, 8>), grid, dim3(512), 0, s, a);
   else if (p.nq == 2) hipLaunchKernelGGL((attn_kv8_rows_kernel<HD, DT, 2, 4>), grid, dim3(256), 0, s, a);
   else if constexpr (HD < 128) hipLaunchKernelGGL((attn_kv8_rows_kernel<HD, DT, 4, 4>), grid, dim3(256), 0, s, a);
   NEKO_CHECK_LAUNCH();
   if (p.splits > 1) {
     const int rows = a.T * a.G, per = 256 / (HD / 4);
-    hipLaunchKernelGGL((attn_kv8_merge_kernel<HD>), dim3((rows + per - 1) / per, a.H, a.S), dim3(256), 0, s, a, p.rtiles * p.nq * 16);
+    hipLaunchKernelGGL((attn_kv8_merge_kernel<HD>), dim3((rows + per - 1) / per, a.H, a.S), dim3(256), 0, s, a, p.rtiles * p.rt);
     NEKO_CHECK_LAUNCH();
   }
   return NEKO_OK;
@@ -355,13 +586,13 @@ int launch_rows(const AttnArgs& a, const Plan& p, hipStream_t s) {
 long neko_attn_kv8_ws_floats_impl(int S, int H, int G, int cap, int hd, int T, int max_len) {
   if (S <= 0 || H <= 0 || G <= 0 || T <= 0 || cap <= 0 || hd <= 0) return 0;
   const Plan p = plan_of(S, H, hd, T * G, max_len > 0 && max_len < cap ? max_len : cap);
-  return p.splits > 1 ? (long)S * H * p.splits * p.rtiles * p.nq * 16 * (hd + 2) : 0;
+  return p.splits > 1 ? (long)S * H * p.splits * p.rtiles * p.rt * (hd + 2) : 0;
 }
 
 int neko_attn_kv8_impl(const uint8_t* k8, const uint8_t* v8, const float* ks, const float* vs, int dtype, int S, int H, int cap, int hd, int block,
                        const bf16_t* q, long q_ss, long q_st, bf16_t* out, long o_ss, long o_st, int G, int T, const int* pos, const int* n_new,
                        const int* start, int window, int sinks, float scale, int max_len, float* ws, long ws_floats, hipStream_t s) {
-  if (!k8 || !v8 || !ks || !vs || !q || !out || !pos || G <= 0 || T <= 0 || window < 0 || sinks < 0) return NEKO_ERR_ARG;
+  if (!k8 || !v8 || !ks || !vs || !q || !out || !pos || G <= 0 || T <= 0 || window < 0 || sinks < 0 || !(scale > 0.f)) return NEKO_ERR_ARG;
   const int rc = neko_kv8_geometry(dtype, S, H, cap, hd, block);
   if (rc) return rc;
   if (T > cap || (long)T * G > (1 << 24)) return NEKO_ERR_ARG;
@@ -373,7 +604,7 @@ int neko_attn_kv8_impl(const uint8_t* k8, const uint8_t* v8, const float* ks, co
   const int bshift = block == 16 ? 4 : block == 32 ? 5 : 6;
   AttnArgs a{k8, v8, ks, vs, q, out, q_ss, q_st, o_ss, o_st, pos, n_new, start, ws, nullptr, S, H, G, cap, T, bshift, window, sinks, p.splits, p.rtiles,
              scale * 1.4426950408889634f};
-  a.part_ml = ws + (long)S * H * p.splits * p.rtiles * p.nq * 16 * hd;
+  a.part_ml = ws + (long)S * H * p.splits * p.rtiles * p.rt * hd;
 #define NEKO_KV8_ATTN(HD) return dtype == 0 ? launch_rows<HD, 0>(a, p, s) : launch_rows<HD, 1>(a, p, s)
   if (hd == 32) NEKO_KV8_ATTN(32);
   if (hd == 64) NEKO_KV8_ATTN(64);

@@ -714,6 +714,7 @@ def attn_kv8(cache: KV8Cache, q: torch.Tensor, pos: torch.Tensor, n_new: Optiona
     T, q_ss, q_st = cache.row_strides(q, HG, "q")
     assert T <= cache.cap, "more rows than the cache has positions"
     assert window >= 0 and sinks >= 0 and (sinks == 0 or window > 0), "sinks need a window"
+    assert scale is None or scale > 0.0, "scale must be positive"
     _here(cache.k, "cache")
     _ints(pos, cache.nseq, "pos")
     _ints(n_new, cache.nseq, "n_new")

@@ -136,11 +136,11 @@ def _attn_case(S, H, G, hd, cap, T, pos, n, start, window, sinks, dtype, block, 
 
 @pytest.mark.parametrize("dtype", [E4, I8], ids=["e4m3", "int8"])
 @pytest.mark.parametrize("hd", [32, 64, 128])
-@pytest.mark.parametrize("T,G", [(1, 1), (1, 4), (6, 3), (7, 8), (70, 1), (40, 3)])
+@pytest.mark.parametrize("T,G", [(1, 1), (1, 4), (6, 3), (7, 8), (70, 1), (40, 3), (150, 2), (300, 1)])
 def test_attn_rows(T, G, hd, dtype):
     """One row, a few, more than one row tile; grouped heads; lengths of one position, of tile borders, at the end of the cache."""
     cap = 320
-    pos = [0, 63 - min(T, 63), 64, 129, cap - T, 200]
+    pos = [0, 63 - min(T, 63), 64, 129, cap - T, 200]             # (long calls run past the end: the rows behind it stay)
     n = [T] * 5 + [max(1, T // 2)]
     _attn_case(6, 2, G, hd, cap, T, pos, n, [0] * 6, 0, 0, dtype, {32: 16, 64: 32, 128: 64}[hd], seed=T + hd)
 

@@ -35,7 +35,7 @@ def test_read_refuses(bad):
 
 
 @pytest.mark.parametrize("bad", BAD_CACHE + [dict(q=None), dict(out=None), dict(pos=None), dict(G=0), dict(T=0), dict(T=65), dict(window=-1), dict(sinks=-1),
-                                             dict(q=P + 2), dict(o_st=63), dict(cap=1 << 16, S=1), dict(G=1 << 24, T=2)], ids=str)
+                                             dict(q=P + 2), dict(o_st=63), dict(scale=0.0), dict(scale=float("nan")), dict(cap=1 << 16, S=1), dict(G=1 << 24, T=2)], ids=str)
 def test_attn_refuses(bad):
     """(the long cache without a workspace among them: its key axis is split)"""
     assert _rc("neko_attn_kv8", {**ATTN, **bad}.values()) in (-1, -2)
