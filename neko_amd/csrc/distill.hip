@@ -41,6 +41,29 @@ template <> struct Piece<bf16_t> {
   static __device__ __forceinline__ uint4 put(const float (&x)[8]) {
     return make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
   }
+  // keeps the first `n` values (n < 8), the others become -inf
+  static __device__ __forceinline__ uint4 mask(const uint4& r, int n) {
+    uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e >= n) w[e >> 1] = (e & 1) ? ((w[e >> 1] & 0x0000ffffu) | 0xff800000u) : ((w[e >> 1] & 0xffff0000u) | 0x0000ff80u);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  // the largest bit pattern as a signed 16-bit integer, two values an instruction: the largest value if that is not negative
+  struct Max {
+    typedef __attribute__((ext_vector_type(2))) short s16x2;
+    s16x2 v = {-32768, -32768};
+    __device__ __forceinline__ void add(const uint4& r) {
+      const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v = __builtin_elementwise_max(v, __builtin_bit_cast(s16x2, w[e]));
+    }
+    __device__ __forceinline__ float value() const {                   // -1 where no value >= 0 was seen (a NaN of either sign stays one or is found later)
+      const short x = v.x > v.y ? v.x : v.y;
+      return x < 0 ? -1.0f : __uint_as_float((uint32_t)(unsigned short)x << 16);
+    }
+    static __device__ __forceinline__ bool is_exact(float m) { return !(m < 0.f); }
+  };
   static __device__ __forceinline__ float one(const bf16_t* p) { return bf16_to_f32(*p); }
   static __device__ __forceinline__ bf16_t store(float x) { return f32_to_bf16(x); }
 };
@@ -52,20 +75,37 @@ template <> struct Piece<float> {
   static __device__ __forceinline__ uint4 put(const float (&x)[4]) {
     return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
   }
+  static __device__ __forceinline__ uint4 mask(const uint4& r, int n) {
+    const uint32_t ni = 0xff800000u;
+    return make_uint4(n > 0 ? r.x : ni, n > 1 ? r.y : ni, n > 2 ? r.z : ni, ni);
+  }
+  struct Max {
+    float v = -INFINITY;
+    __device__ __forceinline__ void add(const uint4& r) {
+      v = fmaxf(v, fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w))));
+    }
+    __device__ __forceinline__ float value() const { return v; }
+    static __device__ __forceinline__ bool is_exact(float) { return true; }
+  };
   static __device__ __forceinline__ float one(const float* p) { return *p; }
   static __device__ __forceinline__ float store(float x) { return x; }
 };
 
-// NCH > 0: the row lives in NCH pieces per thread; 0: it is read again for every use
-template <typename T, int NT, int NCH>
-__global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
+// NCH > 0: the row lives in NCH pieces per thread, as it came (unpacked again in every pass: an unpacked bf16 row would be twice the registers
+// and half the workgroups per CU); 0: it is read again for every use.
+// TWO: labels at temperature 1 beside a teacher at another, two exponentials per element and pass.  The factor of a gradient term is folded into
+// its exponent (2^(c x + b), b = log2 of the factor - c m; -inf for a term that the row does not have): per element 0.5-1 issue slots for the
+// maximum, 7 (13 with TWO) for the sums, 7.5 (12.5) for the gradient, an exponential counting four.
+// two workgroups of 1024 per CU where the row leaves room (64 registers): one loads while the other computes
+template <typename T, int NT, int NCH, bool TWO>
+__global__ __launch_bounds__(NT, NCH <= 7 ? 8 : 4) void distill_kernel(DistillArgs a) {
   using P = Piece<T>;
   constexpr int N = P::N, NW = NT / 64;
-  constexpr float LOG2E = 1.44269504088896340736f;
+  constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
   __shared__ float red[3][NW];
   __shared__ float s_t[KMAX];
   __shared__ int s_i[KMAX];
-  __shared__ float s_teacher[2];                       // soft loss without the student's normaliser; 1 if there is a teacher
+  __shared__ float s_teacher[2];                       // sum t log t; 1 if there is a teacher
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const T* z = (const T*)a.z + (long)row * a.ldz;
   T* dz = a.dz ? (T*)a.dz + (long)row * a.ldd : nullptr;
@@ -84,34 +124,35 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
   // every load of the row is in flight before anything looks at one (clamped, unconditional)
   constexpr int NR = NCH > 0 ? NCH : 1;
   uint4 reg[NR];
+  auto load = [&](int i) {                             // the piece of thread tid, round i; columns >= V are -inf
+    const int c = tid + i * NT;
+    uint4 r = reinterpret_cast<const uint4*>(z)[min(c, nch - 1)];
+    return r;
+  };
+  const int full = a.V / (NT * N);                     // rounds without a column >= V (uniform)
+  auto fence_cols = [&](int i, uint4 r) {
+    const int c = tid + i * NT;
+    if (i >= full && (c + 1) * N > a.V) r = P::mask(r, max(a.V - c * N, 0));
+    return r;
+  };
   if constexpr (NCH > 0) {
 #pragma unroll
-    for (int i = 0; i < NCH; ++i) reg[i] = reinterpret_cast<const uint4*>(z)[min(tid + i * NT, nch - 1)];
+    for (int i = 0; i < NCH; ++i) reg[i] = load(i);
   }
-  // between the passes the row stays packed: without this the compiler keeps every unpacked value instead (twice the registers, spills)
-  auto keep_packed = [&]() {
+  auto keep_packed = [&]() {                           // without this the compiler keeps the unpacked values of the last pass
     if constexpr (NCH > 0) {
 #pragma unroll
       for (int i = 0; i < NCH; ++i) asm volatile("" : "+v"(reg[i].x), "+v"(reg[i].y), "+v"(reg[i].z), "+v"(reg[i].w));
     }
   };
-  // the piece of thread tid, round i, as fp32; columns >= V are -inf
-  auto piece = [&](int i, float (&x)[N]) {
-    const int c = tid + i * NT;
-    P::get(NCH > 0 ? reg[NCH > 0 ? i : 0] : reinterpret_cast<const uint4*>(z)[min(c, nch - 1)], x);
-    if ((c + 1) * N > a.V) {
-#pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (c * N + e >= a.V) x[e] = -INFINITY;
-    }
-  };
   const int rounds = NCH > 0 ? NCH : (nch + NT - 1) / NT;
 
-  // the teacher's entries (wave 0): index, probability, and the student's logit there, read before anything is overwritten
+  // the teacher's entries (wave 0): index, probability
   if (soft_w != 0.f) {
     if (wave == 0) {
       const float it = 1.0f / a.tau;
       float tm = -INFINITY;
+#pragma unroll 1
       for (int j = lane; j < a.k; j += 64) {
         const int ix = a.t_idx[(long)row * a.k + j];
         const float v = ix >= 0 && ix < a.V ? a.t_val[(long)row * a.k + j] : -INFINITY;
@@ -122,11 +163,13 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
       tm = wave_max(tm);
       const bool any = tm != -INFINITY;
       float ts = 0.f;
+#pragma unroll 1
       for (int j = lane; j < a.k; j += 64)
         if (s_i[j] >= 0) ts += __expf((s_t[j] - tm) * it);
       ts = wave_sum(ts);
       const float inv = any ? 1.0f / ts : 0.f, lts = logf(ts);
       float acc = 0.f;
+#pragma unroll 1
       for (int j = lane; j < a.k; j += 64) {
         float t = 0.f;
         if (s_i[j] >= 0) {
@@ -145,61 +188,75 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
   }
 
   // maximum
-  float m = -INFINITY;
+  typename P::Max mx;
 #pragma unroll
   for (int i = 0; i < rounds; ++i) {
-    float x[N];
-    piece(i, x);
-#pragma unroll
-    for (int e = 0; e < N; ++e) m = fmaxf(m, x[e]);
+    if constexpr (NCH > 0) { reg[i] = fence_cols(i, reg[i]); mx.add(reg[i]); }
+    else mx.add(fence_cols(i, load(i)));
   }
-  m = wave_max(m);
+  float m = wave_max(mx.value());
   if (lane == 0) red[0][wave] = m;
   __syncthreads();
   m = red[0][0];
 #pragma unroll
   for (int i = 1; i < NW; ++i) m = fmaxf(m, red[0][i]);
+  if (!P::Max::is_exact(m)) {                          // bf16, no value >= 0 in the row: its largest by value
+    __syncthreads();
+    m = -INFINITY;
+#pragma unroll 1
+    for (int i = 0; i < rounds; ++i) {
+      float x[N];
+      P::get(fence_cols(i, load(i)), x);
+#pragma unroll
+      for (int e = 0; e < N; ++e) m = fmaxf(m, x[e]);
+    }
+    m = wave_max(m);
+    if (lane == 0) red[0][wave] = m;
+    __syncthreads();
+    m = red[0][0];
+#pragma unroll
+    for (int i = 1; i < NW; ++i) m = fmaxf(m, red[0][i]);
+  }
 
-  // sums, at the temperature and (for the labels) without it
+  // sums: c1 serves the teacher's temperature (and the labels where that is 1 or there is no teacher), LOG2E the labels' with TWO
   const bool soft = soft_w != 0.f && s_teacher[1] != 0.f;
-  const float c_soft = LOG2E / a.tau;
-  const bool two = has_y && a.tau != 1.0f && soft;
-  const float c_one = soft ? c_soft : LOG2E;
+  const float c1 = soft_w != 0.f ? LOG2E / a.tau : LOG2E;
+  // 2^(c x - n), n = c m rounded to an integer: the fused multiply-add then rounds once, relative to the exponent itself
+  const float b1 = -rintf(m * c1), b2 = -rintf(m * LOG2E);
   float s1 = 0.f, s2 = 0.f;
   keep_packed();
 #pragma unroll
   for (int i = 0; i < rounds; ++i) {
     float x[N];
-    piece(i, x);
+    if constexpr (NCH > 0) P::get(reg[i], x);
+    else P::get(fence_cols(i, load(i)), x);
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      const float d = x[e] - m;
-      s1 += __builtin_amdgcn_exp2f(d * c_one);
-      if (two) s2 += __builtin_amdgcn_exp2f(d * LOG2E);
+      s1 += __builtin_amdgcn_exp2f(fmaf(x[e], c1, b1));
+      if (TWO) s2 += __builtin_amdgcn_exp2f(fmaf(x[e], LOG2E, b2));
     }
   }
   s1 = wave_sum(s1);
-  if (two) s2 = wave_sum(s2);
+  if (TWO) s2 = wave_sum(s2);
   if (lane == 0) { red[1][wave] = s1; red[2][wave] = s2; }
-  // the sparse places of this thread: teacher entries, then the label
   __syncthreads();
   s1 = s2 = 0.f;
 #pragma unroll
   for (int i = 0; i < NW; ++i) { s1 += red[1][i]; s2 += red[2][i]; }
-  const float sum_soft = s1, sum_hard = two ? s2 : s1;
-  const float gs = soft ? w * soft_w * a.tau / sum_soft : 0.f;      // dense terms: gs 2^(c_soft d) + gh 2^(LOG2E d)
-  const float gh = has_y ? w * a.hard / sum_hard : 0.f;
+  const float sum_soft = s1, sum_hard = TWO ? s2 : s1;
+  const float fs = soft ? soft_w * a.tau / sum_soft : 0.f, fh = has_y ? a.hard / sum_hard : 0.f;
 
   if (wave == 0 && a.loss_row) {
     float acc = 0.f;
     if (soft)
+#pragma unroll 1
       for (int j = lane; j < a.k; j += 64)
-        if (s_t[j] > 0.f) acc += s_t[j] * (P::one(z + s_i[j]) - m);
+        if (s_t[j] > 0.f) acc += s_t[j] * fmaf(P::one(z + s_i[j]), c1, b1);
     acc = wave_sum(acc);
     if (lane == 0) {
       float loss = 0.f;
-      if (soft) loss += soft_w * a.tau * a.tau * (s_teacher[0] - acc / a.tau + logf(sum_soft));
-      if (has_y) loss += a.hard * (logf(sum_hard) - (P::one(z + y) - m));
+      if (soft) loss += soft_w * a.tau * a.tau * (s_teacher[0] + LN2 * (log2f(sum_soft) - acc));
+      if (has_y) loss += a.hard * LN2 * (log2f(sum_hard) - (TWO ? fmaf(P::one(z + y), LOG2E, b2) : fmaf(P::one(z + y), c1, b1)));
       a.loss_row[row] = loss;
     }
   }
@@ -216,35 +273,50 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
     if (j < a.k && soft) at[q] = s_i[j];
     if (j == a.k && has_y) at[q] = (int)y;
     if (at[q] >= 0) {
-      const float d = P::one(z + at[q]) - m;
+      const float x = P::one(z + at[q]);
       float t = 0.f;
       if (soft)
+#pragma unroll 4
         for (int i = 0; i < a.k; ++i) t += s_i[i] == at[q] ? s_t[i] : 0.f;
       float g = 0.f;
-      if (soft) g += w * soft_w * a.tau * (__builtin_amdgcn_exp2f(d * c_soft) / sum_soft - t);
-      if (has_y) g += w * a.hard * (__builtin_amdgcn_exp2f(d * LOG2E) / sum_hard - (at[q] == (int)y ? 1.f : 0.f));
+      if (soft) g += w * (fs * __builtin_amdgcn_exp2f(fmaf(x, c1, b1)) - soft_w * a.tau * t);
+      if (has_y) g += w * (fh * __builtin_amdgcn_exp2f(TWO ? fmaf(x, LOG2E, b2) : fmaf(x, c1, b1)) - (at[q] == (int)y ? a.hard : 0.f));
       fix[q] = g;
     }
   }
   __syncthreads();                                      // every sparse logit is read
   keep_packed();
+  // bf16 results: the factor of a term goes into its exponent, the sign of the weight into the packing.  fp32 results multiply (an exponent of 40
+  // is held to 2^-19 only)
+  constexpr bool FOLD = sizeof(T) == 2;
+  const float f1 = w * (TWO ? fs : fs + fh), f2 = w * fh;
+  const float e1 = FOLD ? b1 + __log2f(fabsf(f1)) : b1, e2 = FOLD ? b2 + __log2f(fabsf(f2)) : b2;
+  const bool neg = FOLD && w < 0.f;
 #pragma unroll
   for (int i = 0; i < rounds; ++i) {
     const int c = tid + i * NT;
     float x[N];
-    piece(i, x);
+    if constexpr (NCH > 0) P::get(reg[i], x);
+    else P::get(fence_cols(i, load(i)), x);
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      const float d = x[e] - m;
-      float g = 0.f;
-      if (soft && has_y && !two) g = __builtin_amdgcn_exp2f(d * LOG2E) * (gs + gh);       // one temperature: one exponential
-      else {
-        if (soft) g = __builtin_amdgcn_exp2f(d * c_soft) * gs;
-        if (has_y) g = fmaf(__builtin_amdgcn_exp2f(d * LOG2E), gh, g);
+      float g = __builtin_amdgcn_exp2f(fmaf(x[e], c1, e1));
+      if (!FOLD) g *= f1;
+      if (TWO) {
+        const float g2 = __builtin_amdgcn_exp2f(fmaf(x[e], LOG2E, e2));
+        g = FOLD ? g + g2 : fmaf(g2, f2, g);
       }
-      x[e] = c * N + e < a.V ? g : 0.f;
+      x[e] = g;
     }
-    if (c < nch) reinterpret_cast<uint4*>(dz)[c] = P::put(x);
+    if (neg) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) x[e] = -x[e];
+    }
+    if (c < nch) {
+      typedef __attribute__((ext_vector_type(4))) uint32_t u32x4_v;
+      const uint4 o = P::put(x);
+      __builtin_nontemporal_store((u32x4_v){o.x, o.y, o.z, o.w}, reinterpret_cast<u32x4_v*>(dz) + c);
+    }
   }
   __syncthreads();                                      // the dense values are written
 #pragma unroll
@@ -255,7 +327,12 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
 template <typename T>
 int launch(const DistillArgs& a, int R, hipStream_t s) {
   const int nch = a.Vpad / Piece<T>::N;
-#define NEKO_DISTILL(NT, NCH) hipLaunchKernelGGL((distill_kernel<T, NT, NCH>), dim3(R), dim3(NT), 0, s, a)
+  const bool two = a.hard > 0.f && a.hard < 1.f && a.tau != 1.0f;
+#define NEKO_DISTILL(NT, NCH)                                                                              \
+  do {                                                                                                     \
+    if (two) hipLaunchKernelGGL((distill_kernel<T, NT, NCH, true>), dim3(R), dim3(NT), 0, s, a);           \
+    else hipLaunchKernelGGL((distill_kernel<T, NT, NCH, false>), dim3(R), dim3(NT), 0, s, a);              \
+  } while (0)
   if (nch <= 256) NEKO_DISTILL(256, 1);                 // short vocabularies: small workgroups, several rows per CU
   else if (nch <= 1024) NEKO_DISTILL(256, 4);
   else if (nch <= 4 * 1024) NEKO_DISTILL(1024, 4);
