@@ -8,7 +8,8 @@
 // tau = 0: x_i is kept while it is the target row's largest logit (lowest index among equals), the next token is the largest of row a.
 //
 // The answer is an index: a sum over 50 thousand tokens that ends next to the border picks another token in 32 bits once in a few hundred
-// calls, so weights and sums are fp64 -- with an exponential of its own (exp64 below).
+// calls, so weights and sums are fp64 -- with an exponential of its own (pow2_64: 17 instructions an element at the fp64 rate, which hides behind
+// the memory).
 // Reads (2 K + 1) V logits once (HBM), then the two rows that are sampled from again (last-level cache).  Three launches: row pieces ->
 // (maximum, sum); acceptance, redone by every workgroup from the pieces, and the sampled weights' sum per piece; the piece that holds the
 // border and the token in it.  tau = 0 needs two.
@@ -19,6 +20,7 @@ namespace {
 constexpr int VT = 256, VE = 16, PIECE = VT * VE;      // 4096 logits per workgroup, 16 a thread
 constexpr int MAXK = 63;                               // a lane per drafted token
 
+struct Source;
 struct VerifyArgs {
   const void *target, *draft;
   long t_sb, t_sr, d_sb, d_sr;
@@ -29,9 +31,10 @@ struct VerifyArgs {
   long long* out;
   float* pm;          // [B][2K+1][pieces] maximum of the piece
   double* ps;         // sum of exp((l - piece maximum) / tau); tau = 0: the index of the maximum
-  double* pw;         // [B][pieces] sums of the sampled weights
+  double* pw;         // [B][pieces][2] sums of the sampled weights: the residual's, the target's own
+  Source* src; // [B]
   int B, K, V, pieces;
-  double inv_tau;
+  double c;           // log2(e) / tau
   int greedy;
 };
 
@@ -39,36 +42,48 @@ template <typename T> __device__ __forceinline__ float logit(const T* p, long i)
 template <> __device__ __forceinline__ float logit<float>(const float* p, long i) { const float x = p[i]; return x == x ? x : -INFINITY; }
 template <> __device__ __forceinline__ float logit<bf16_t>(const bf16_t* p, long i) { const float x = bf16_to_f32(p[i]); return x == x ? x : -INFINITY; }
 
-// e^x for x <= 0, fp64: x = n ln 2 + f (ln 2 as its nearest double and the rest, both steps fused), Taylor series of e^f to f^13 / 13!
-// (|f| <= 0.3466: the next term is 4e-18), scaled by 2^n; below -708: 0
-__device__ __forceinline__ double exp64(double x) {
-  const double n = rint(x * 1.4426950408889634074);
-  double f = fma(n, -0.693147180559945309417, x);
-  f = fma(n, -2.3190468138462996e-17, f);
-  double p = 1.0 / 6227020800.0;
-  p = fma(p, f, 1.0 / 479001600.0);
-  p = fma(p, f, 1.0 / 39916800.0);
-  p = fma(p, f, 1.0 / 3628800.0);
-  p = fma(p, f, 1.0 / 362880.0);
-  p = fma(p, f, 1.0 / 40320.0);
-  p = fma(p, f, 1.0 / 5040.0);
-  p = fma(p, f, 1.0 / 720.0);
-  p = fma(p, f, 1.0 / 120.0);
-  p = fma(p, f, 1.0 / 24.0);
-  p = fma(p, f, 1.0 / 6.0);
-  p = fma(p, f, 0.5);
+// 2^x for x <= 1/2, fp64: x = n + f, Taylor series of e^(f ln 2) to the 11th power (|f| <= 1/2: the next term is 6e-15), scaled by 2^n; below -1100: 0
+__device__ __forceinline__ double pow2_64(double x) {
+  x = fmax(x, -1100.0);
+  const double n = rint(x), f = x - n;
+  constexpr double L = 0.693147180559945309417;
+  constexpr double L2 = L * L, L3 = L2 * L, L4 = L2 * L2, L5 = L4 * L, L6 = L3 * L3, L7 = L6 * L, L8 = L4 * L4, L9 = L8 * L, L10 = L5 * L5, L11 = L10 * L;
+  double p = L11 / 39916800.0;
+  p = fma(p, f, L10 / 3628800.0);
+  p = fma(p, f, L9 / 362880.0);
+  p = fma(p, f, L8 / 40320.0);
+  p = fma(p, f, L7 / 5040.0);
+  p = fma(p, f, L6 / 720.0);
+  p = fma(p, f, L5 / 120.0);
+  p = fma(p, f, L4 / 24.0);
+  p = fma(p, f, L3 / 6.0);
+  p = fma(p, f, L2 / 2.0);
+  p = fma(p, f, L);
   p = fma(p, f, 1.0);
-  p = fma(p, f, 1.0);
-  return x < -708.0 ? 0.0 : ldexp(p, (int)n);
+  return ldexp(p, (int)n);
 }
-// weight of logit l under maximum m: equal logits weigh 1 also where both are infinite
-__device__ __forceinline__ double weight(float l, float m, double inv_tau) {
-  if (l == m) return m == -INFINITY ? 0.0 : 1.0;
-  return exp64(((double)l - (double)m) * inv_tau);
-}
+// weight of logit l under the maximum m, c = log2(e) / tau: 2^(c l - c m); an infinite maximum shares the mass among its equals
+struct Weigh {
+  double c, cm;
+  float m;
+  bool inf;
+  __device__ __forceinline__ Weigh(float m_, double c_) : c(c_), cm((double)m_ * c_), m(m_), inf(m_ == INFINITY || m_ == -INFINITY) {}
+  __device__ __forceinline__ double operator()(float l) const {
+    if (inf) return l == m && m == INFINITY ? 1.0 : 0.0;
+    return pow2_64(fma((double)l, c, -cm));
+  }
+};
 __device__ __forceinline__ double wave_sum64(double v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+__device__ __forceinline__ double wave_scan64(double v, int lane) {       // inclusive
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double u = __shfl_up(v, o, 64);
+    if (lane >= o) v += u;
+  }
   return v;
 }
 __device__ __forceinline__ int drafted(const VerifyArgs& a, int b) { return min(max(a.n_draft ? a.n_draft[b] : a.K, 0), a.K); }
@@ -102,7 +117,7 @@ __global__ __launch_bounds__(VT) void verify_rows_kernel(VerifyArgs a) {
   float wm = wave_max(m);
   if (lane == 0) sm[wave] = wm;
   __syncthreads();
-  float bm = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+  const float bm = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
   const long o = ((long)b * (2 * a.K + 1) + row) * a.pieces + piece;
   if (a.greedy) {
     int idx = m == bm ? at : 0x7fffffff;                              // lowest index among equals
@@ -113,114 +128,118 @@ __global__ __launch_bounds__(VT) void verify_rows_kernel(VerifyArgs a) {
     if (threadIdx.x == 0) { a.pm[o] = bm; a.ps[o] = (double)min(min(si[0], si[1]), min(si[2], si[3])); }
     return;
   }
+  const Weigh w(bm, a.c);
   double s = 0.0;
 #pragma unroll
-  for (int e = 0; e < VE; ++e) s += weight(x[e], bm, a.inv_tau);
+  for (int e = 0; e < VE; ++e) s += w(x[e]);
   s = wave_sum64(s);
   if (lane == 0) ss[wave] = s;
   __syncthreads();
   if (threadIdx.x == 0) { a.pm[o] = bm; a.ps[o] = (ss[0] + ss[1]) + (ss[2] + ss[3]); }
 }
 
-// a row's maximum and sum from its pieces
-__device__ __forceinline__ void row_stats(const VerifyArgs& a, int b, int row, float& m, double& s) {
-  const long o = ((long)b * (2 * a.K + 1) + row) * a.pieces;
-  m = -INFINITY;
-  for (int p = 0; p < a.pieces; ++p) m = fmaxf(m, a.pm[o + p]);
-  s = 0.0;
-  for (int p = 0; p < a.pieces; ++p) s += a.ps[o + p] * weight(a.pm[o + p], m, a.inv_tau);
+// What is sampled from once `kept` are kept: target row and maximum and 1 / sum, and the draft row's that is taken off (or one token).
+struct Source { float mp, mq; double ip, iq; int has_q; int x; };
+
+template <typename T>
+__device__ __forceinline__ double residual(float lp, float lq, int c, const Source& s, const Weigh& wp, const Weigh& wq, double& own) {
+  own = wp(lp) * s.ip;
+  if (s.has_q) return fmax(own - wq(lq) * s.iq, 0.0);
+  return c == s.x ? 0.0 : own;
 }
 
-// lane i of a wave judges draft i; returns the number kept (every lane)
-template <typename T>
-__device__ __forceinline__ int accept(const VerifyArgs& a, int b, int n, int lane) {
-  bool ok = false;
-  if (lane < n) {
-    float mp, mq;
-    double sp, sq;
-    row_stats(a, b, lane, mp, sp);
-    const long long x = a.tokens[(long)b * a.K + lane];
-    if (x >= 0 && x < a.V) {
-      const double p = weight(logit<T>((const T*)a.target + a.t_sb * b + a.t_sr * lane, x), mp, a.inv_tau) / sp;
-      double q = 1.0;
-      if (a.draft) {
-        row_stats(a, b, a.K + 1 + lane, mq, sq);
-        q = weight(logit<T>((const T*)a.draft + a.d_sb * b + a.d_sr * lane, x), mq, a.inv_tau) / sq;
-      }
-      ok = (double)a.u[(long)b * a.K + lane] * q < p;
-    }
-  }
-  const unsigned long long bad = ~__builtin_amdgcn_ballot_w64(ok);
-  return min(n, __builtin_ctzll(bad | (1ull << 63)));
-}
-
-// What is sampled from once `kept` are kept: the target row, and the draft row that is taken off (if any).
-template <typename T>
-struct Source {
-  const T *p, *q;
-  long long x;        // without draft logits: the token that is taken off, or -1
-  float mp, mq;
-  double ip, iq;      // 1 / sum
-  __device__ __forceinline__ Source(const VerifyArgs& a, int b, int n, int kept) {
-    double s;
-    p = (const T*)a.target + a.t_sb * b + a.t_sr * kept;
-    row_stats(a, b, kept, mp, s);
-    ip = s > 0.0 ? 1.0 / s : 0.0;
-    q = nullptr;
-    x = -1;
-    mq = 0.f;
-    iq = 0.0;
-    if (kept < n) {
-      if (a.draft) {
-        q = (const T*)a.draft + a.d_sb * b + a.d_sr * kept;
-        row_stats(a, b, a.K + 1 + kept, mq, s);
-        iq = s > 0.0 ? 1.0 / s : 0.0;
-      } else {
-        x = a.tokens[(long)b * a.K + kept];
-      }
-    }
-  }
-  // residual weight and the target's own
-  __device__ __forceinline__ double operator()(const VerifyArgs& a, int c, double& own) const {
-    own = weight(logit<T>(p, c), mp, a.inv_tau) * ip;
-    if (q) return fmax(own - weight(logit<T>(q, c), mq, a.inv_tau) * iq, 0.0);
-    return c == x ? 0.0 : own;
-  }
-};
-
-// ---- launch 2: acceptance, and per piece the sums of the sampled weights (greedy: everything) ----
+// ---- launch 2: acceptance (by every workgroup again, from the pieces), and the sums of the sampled weights of one piece ----
 template <typename T>
 __global__ __launch_bounds__(VT) void verify_accept_kernel(VerifyArgs a) {
   __shared__ double ss[VT / 64][2];
+  __shared__ float row_m[2 * MAXK];
+  __shared__ double row_s[2 * MAXK];
+  __shared__ Source s_src;
   __shared__ int s_kept;
   const int piece = blockIdx.x, b = blockIdx.y;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int n = drafted(a, b);
-  if (wave == 0) {
-    const int kept = accept<T>(a, b, n, lane);
-    if (lane == 0) s_kept = kept;
+  // rows 0..n of the target, then n of the draft: sixteen lanes each
+  const int nrows = a.draft ? 2 * n + 1 : n + 1;
+  for (int q = tid >> 4; q < nrows; q += VT / 16) {
+    const int row = q <= n ? q : a.K + 1 + (q - n - 1);
+    const long o = ((long)b * (2 * a.K + 1) + row) * a.pieces;
+    float m = -INFINITY;
+    for (int p = lane & 15; p < a.pieces; p += 16) m = fmaxf(m, a.pm[o + p]);
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+    const Weigh w(m, a.c);
+    double s = 0.0;
+    for (int p = lane & 15; p < a.pieces; p += 16) s += a.ps[o + p] * w(a.pm[o + p]);
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) s += __shfl_xor(s, d, 64);
+    if ((lane & 15) == 0) { row_m[q] = m; row_s[q] = s; }
+  }
+  __syncthreads();
+  if (wave == 0) {                                                    // lane i judges draft i
+    bool ok = false;
+    if (lane < n) {
+      const long long x = a.tokens[(long)b * a.K + lane];
+      if (x >= 0 && x < a.V) {
+        const float u = a.u[(long)b * a.K + lane];
+        const float lp = logit<T>((const T*)a.target + a.t_sb * b + a.t_sr * lane, x);
+        const float lq = a.draft ? logit<T>((const T*)a.draft + a.d_sb * b + a.d_sr * lane, x) : 0.f;
+        const double p = Weigh(row_m[lane], a.c)(lp) / row_s[lane];
+        const double q = a.draft ? Weigh(row_m[n + 1 + lane], a.c)(lq) / row_s[n + 1 + lane] : 1.0;
+        ok = (double)u * q < p;
+      }
+    }
+    const unsigned long long bad = ~__builtin_amdgcn_ballot_w64(ok);
+    const int kept = min(n, (int)__builtin_ctzll(bad | (1ull << 63)));
+    if (lane == 0) {
+      Source s{row_m[kept], 0.f, row_s[kept] > 0.0 ? 1.0 / row_s[kept] : 0.0, 0.0, 0, -1};
+      if (kept < n) {
+        if (a.draft) {
+          s.has_q = 1;
+          s.mq = row_m[n + 1 + kept];
+          s.iq = row_s[n + 1 + kept] > 0.0 ? 1.0 / row_s[n + 1 + kept] : 0.0;
+        } else {
+          const long long x = a.tokens[(long)b * a.K + kept];
+          s.x = x >= 0 && x < a.V ? (int)x : -1;
+        }
+      }
+      s_src = s;
+      s_kept = kept;
+      if (piece == 0) {
+        a.accepted[b] = kept;
+        a.src[b] = s;
+      }
+    }
   }
   __syncthreads();
   const int kept = s_kept;
-  const Source<T> src(a, b, n, kept);
-  double sr = 0.0, so = 0.0;
+  const Source src = s_src;
+  const T* zp = (const T*)a.target + a.t_sb * b + a.t_sr * kept;
+  const T* zq = src.has_q ? (const T*)a.draft + a.d_sb * b + a.d_sr * kept : zp;
+  float lp[VE], lq[VE];
+#pragma unroll
   for (int e = 0; e < VE; ++e) {
-    const int c = piece * PIECE + e * VT + (int)threadIdx.x;
-    if (c < a.V) {
-      double own;
-      sr += src(a, c, own);
-      so += own;
-    }
+    const int c = min(piece * PIECE + e * VT + tid, a.V - 1);
+    lp[e] = logit<T>(zp, c);
+    lq[e] = logit<T>(zq, c);
+  }
+  const Weigh wp(src.mp, a.c), wq(src.mq, a.c);
+  double sr = 0.0, so = 0.0;
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    const int c = piece * PIECE + e * VT + tid;
+    double own;
+    const double res = residual<T>(lp[e], lq[e], c, src, wp, wq, own);
+    if (c < a.V) { sr += res; so += own; }
   }
   sr = wave_sum64(sr);
   so = wave_sum64(so);
   if (lane == 0) { ss[wave][0] = sr; ss[wave][1] = so; }
   __syncthreads();
-  if (threadIdx.x == 0) {
+  if (tid == 0) {
     double* w = a.pw + ((long)b * a.pieces + piece) * 2;
     w[0] = (ss[0][0] + ss[1][0]) + (ss[2][0] + ss[3][0]);
     w[1] = (ss[0][1] + ss[1][1]) + (ss[2][1] + ss[3][1]);
-    if (piece == 0) a.accepted[b] = kept;
   }
 }
 
@@ -229,81 +248,107 @@ __device__ __forceinline__ void write_tokens(const VerifyArgs& a, int b, int kep
     a.out[(long)b * (a.K + 1) + i] = i < kept ? a.tokens[(long)b * a.K + i] : i == kept ? next : -1;
 }
 
-__global__ __launch_bounds__(64) void verify_greedy_kernel(VerifyArgs a) {
-  const int b = blockIdx.x, lane = threadIdx.x;
+// greedy, launch 2: sixteen lanes find the best token of a row; then the chain
+__global__ __launch_bounds__(VT) void verify_greedy_kernel(VerifyArgs a) {
+  __shared__ int best[MAXK + 1];
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   const int n = drafted(a, b);
-  long long best = -1;
-  bool ok = false;
-  if (lane <= n) {
-    const long o = ((long)b * (2 * a.K + 1) + lane) * a.pieces;
+  for (int q = tid >> 4; q <= n; q += VT / 16) {
+    const long o = ((long)b * (2 * a.K + 1) + q) * a.pieces;
     float m = -INFINITY;
-    for (int p = 0; p < a.pieces; ++p)
-      if (a.pm[o + p] > m) { m = a.pm[o + p]; best = (long long)a.ps[o + p]; }
-    ok = lane < n && best >= 0 && best == a.tokens[(long)b * a.K + lane];
+    int at = 0x7fffffff;
+    for (int p = lane & 15; p < a.pieces; p += 16) {
+      const float x = a.pm[o + p];
+      const int i = (int)a.ps[o + p];
+      if (x > m) { m = x; at = i; }
+    }
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) {
+      const float om = __shfl_xor(m, d, 64);
+      const int oa = __shfl_xor(at, d, 64);
+      if (om > m || (om == m && oa < at)) { m = om; at = oa; }
+    }
+    if ((lane & 15) == 0) best[q] = m == -INFINITY ? -1 : at;
   }
-  const unsigned long long bad = ~__builtin_amdgcn_ballot_w64(ok);
-  const int kept = min(n, __builtin_ctzll(bad | (1ull << 63)));
-  const long long next = __shfl(best, kept, 64);
-  write_tokens(a, b, kept, next);
-  if (lane == 0) a.accepted[b] = kept;
+  __syncthreads();
+  if (tid < 64) {
+    const bool ok = lane < n && best[lane] >= 0 && best[lane] == a.tokens[(long)b * a.K + lane];
+    const unsigned long long bad = ~__builtin_amdgcn_ballot_w64(ok);
+    const int kept = min(n, (int)__builtin_ctzll(bad | (1ull << 63)));
+    const long long next = best[kept];
+    for (int i = lane; i <= a.K; i += 64) a.out[(long)b * (a.K + 1) + i] = i < kept ? a.tokens[(long)b * a.K + i] : i == kept ? next : -1;
+    if (lane == 0) a.accepted[b] = kept;
+  }
 }
 
 // ---- launch 3: the piece that holds the border, and the token in it ----
 template <typename T>
 __global__ __launch_bounds__(VT) void verify_sample_kernel(VerifyArgs a) {
-  __shared__ double part[VT];
+  __shared__ double f[PIECE + PIECE / VE];                // a thread's sixteen consecutive weights, padded by one
+  __shared__ double wsum[VT / 64];
   __shared__ int s_at, s_last;
-  const int b = blockIdx.x, tid = threadIdx.x;
-  const int n = drafted(a, b), kept = a.accepted[b];
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int kept = a.accepted[b];
+  const Source src = a.src[b];
   const double* w = a.pw + (long)b * a.pieces * 2;
-  double total = 0.0;
-  for (int p = 0; p < a.pieces; ++p) total += w[2 * p];
-  const int col = total > 0.0 ? 0 : 1;                    // nothing is left of p - q: the target's own distribution
-  if (col) {
-    total = 0.0;
-    for (int p = 0; p < a.pieces; ++p) total += w[2 * p + 1];
-  }
+  // every wave finds the piece: totals, then the first piece whose running sum passes the border
+  double t0 = 0.0, t1 = 0.0;
+  for (int p = lane; p < a.pieces; p += 64) { t0 += w[2 * p]; t1 += w[2 * p + 1]; }
+  t0 = wave_sum64(t0);
+  const int col = t0 > 0.0 ? 0 : 1;                       // nothing is left of p - q: the target's own distribution
+  const double total = col ? wave_sum64(t1) : t0;
   if (!(total > 0.0)) {                                   // a row without a finite logit
     write_tokens(a, b, kept, -1);
     return;
   }
   const double border = (double)a.r[b] * total;
   int piece = -1;
-  double before = 0.0;
-  for (int p = 0; p < a.pieces; ++p) {
-    const double x = w[2 * p + col];
-    if (x > 0.0) {
-      if (piece >= 0) before += w[2 * piece + col];       // the last piece with weight stays where rounding leaves none above the border
-      piece = p;
-      if (before + x > border) break;
+  double before = 0.0, run0 = 0.0;
+  for (int p0 = 0; p0 < a.pieces; p0 += 64) {
+    const double x = p0 + lane < a.pieces ? w[2 * (p0 + lane) + col] : 0.0;
+    const double incl = run0 + wave_scan64(x, lane);
+    const unsigned long long some = __builtin_amdgcn_ballot_w64(x > 0.0), over = __builtin_amdgcn_ballot_w64(x > 0.0 && incl > border);
+    // without a piece above the border (rounding, r next to 1) the last one with weight stands
+    const int pick = over ? (int)__builtin_ctzll(over) : some ? 63 - (int)__builtin_clzll(some) : -1;
+    if (pick >= 0) {
+      piece = p0 + pick;
+      before = __shfl(incl - x, pick, 64);
+      if (over) break;
     }
+    run0 = __shfl(incl, 63, 64);
   }
-  const Source<T> src(a, b, n, kept);
-  const int c0 = piece * PIECE + tid * VE;                // here a thread holds 16 consecutive tokens
-  double f[VE], sum = 0.0;
+  const T* zp = (const T*)a.target + a.t_sb * b + a.t_sr * kept;
+  const T* zq = src.has_q ? (const T*)a.draft + a.d_sb * b + a.d_sr * kept : zp;
+  const Weigh wp(src.mp, a.c), wq(src.mq, a.c);
+  float lp[VE], lq[VE];
+#pragma unroll
   for (int e = 0; e < VE; ++e) {
-    f[e] = 0.0;
-    if (c0 + e < a.V) {
-      double own;
-      const double res = src(a, c0 + e, own);
-      f[e] = col ? own : res;
-    }
-    sum += f[e];
+    const int c = min(piece * PIECE + e * VT + tid, a.V - 1);
+    lp[e] = logit<T>(zp, c);
+    lq[e] = logit<T>(zq, c);
   }
-  part[tid] = sum;
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    const int i = e * VT + tid, c = piece * PIECE + i;
+    double own;
+    const double res = residual<T>(lp[e], lq[e], c, src, wp, wq, own);
+    f[i + i / VE] = c < a.V ? (col ? own : res) : 0.0;
+  }
   if (tid == 0) { s_at = 0x7fffffff; s_last = -1; }
   __syncthreads();
-  for (int d = 1; d < VT; d <<= 1) {                      // inclusive scan
-    const double v = tid >= d ? part[tid - d] : 0.0;
-    __syncthreads();
-    part[tid] += v;
-    __syncthreads();
-  }
-  double run = before + (tid ? part[tid - 1] : 0.0);
+  double sum = 0.0;
+  for (int e = 0; e < VE; ++e) sum += f[tid * (VE + 1) + e];
+  const double incl = wave_scan64(sum, lane);
+  if (lane == 63) wsum[wave] = incl;
+  __syncthreads();
+  double run = before + (incl - sum);
+  for (int i = 0; i < wave; ++i) run += wsum[i];
+  const int c0 = piece * PIECE + tid * VE;
   int at = 0x7fffffff, last = -1;
   for (int e = 0; e < VE; ++e) {
-    run += f[e];
-    if (f[e] > 0.0) {
+    const double x = f[tid * (VE + 1) + e];
+    run += x;
+    if (x > 0.0) {
       last = c0 + e;
       if (run > border && at == 0x7fffffff) at = c0 + e;
     }
@@ -320,7 +365,7 @@ int launch(const VerifyArgs& a, hipStream_t s) {
   hipLaunchKernelGGL((verify_rows_kernel<T>), dim3(a.pieces, rows, a.B), dim3(VT), 0, s, a);
   NEKO_CHECK_LAUNCH();
   if (a.greedy) {
-    hipLaunchKernelGGL(verify_greedy_kernel, dim3(a.B), dim3(64), 0, s, a);
+    hipLaunchKernelGGL(verify_greedy_kernel, dim3(a.B), dim3(VT), 0, s, a);
   } else {
     hipLaunchKernelGGL((verify_accept_kernel<T>), dim3(a.pieces, a.B), dim3(VT), 0, s, a);
     NEKO_CHECK_LAUNCH();
@@ -335,7 +380,7 @@ int launch(const VerifyArgs& a, hipStream_t s) {
 long neko_verify_draft_ws_bytes_impl(int B, int K, int V) {
   if (B <= 0 || K <= 0 || V <= 0) return 0;
   const long pieces = (V + PIECE - 1) / PIECE;
-  return (long)B * pieces * ((2 * K + 1) * 12L + 16L) + 16;
+  return (long)B * pieces * ((2 * K + 1) * 12L + 16L) + (long)B * (long)sizeof(Source);
 }
 
 int neko_verify_draft_impl(const void* target, long t_sb, long t_sr, const void* draft, long d_sb, long d_sr, int is_bf16, int B, int K, int V,
@@ -352,8 +397,9 @@ int neko_verify_draft_impl(const void* target, long t_sb, long t_sr, const void*
   const long cells = (long)B * (2 * K + 1) * a.pieces;
   a.ps = (double*)ws;
   a.pw = a.ps + cells;
-  a.pm = (float*)(a.pw + 2L * B * a.pieces);
+  a.src = (Source*)(a.pw + 2L * B * a.pieces);
+  a.pm = (float*)(a.src + B);
   a.greedy = temperature == 0.f;
-  a.inv_tau = a.greedy ? 1.0 : 1.0 / (double)temperature;
+  a.c = a.greedy ? 1.0 : 1.4426950408889634074 / (double)temperature;
   return is_bf16 ? launch<bf16_t>(a, s) : launch<float>(a, s);
 }
