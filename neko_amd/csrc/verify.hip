@@ -8,8 +8,7 @@
 // tau = 0: x_i is kept while it is the target row's largest logit (lowest index among equals), the next token is the largest of row a.
 //
 // The answer is an index: a sum over 50 thousand tokens that ends next to the border picks another token in 32 bits once in a few hundred
-// calls, so weights and sums are fp64 -- with an exponential of its own (pow2_64: 17 instructions an element at the fp64 rate, which hides behind
-// the memory).
+// calls, so weights and sums are fp64 -- with an exponential of its own (pow2_64).
 // Reads (2 K + 1) V logits once (HBM), then the two rows that are sampled from again (last-level cache).  Three launches: row pieces ->
 // (maximum, sum); acceptance, redone by every workgroup from the pieces, and the sampled weights' sum per piece; the piece that holds the
 // border and the token in it.  tau = 0 needs two.
@@ -42,25 +41,23 @@ template <typename T> __device__ __forceinline__ float logit(const T* p, long i)
 template <> __device__ __forceinline__ float logit<float>(const float* p, long i) { const float x = p[i]; return x == x ? x : -INFINITY; }
 template <> __device__ __forceinline__ float logit<bf16_t>(const bf16_t* p, long i) { const float x = bf16_to_f32(p[i]); return x == x ? x : -INFINITY; }
 
-// 2^x for x <= 1/2, fp64: x = n + f, Taylor series of e^(f ln 2) to the 11th power (|f| <= 1/2: the next term is 6e-15), scaled by 2^n; below -1100: 0
+// 2^x for x <= 1/2, fp64: x = n + f, the polynomial of degree 9 that interpolates 2^f at the ten Chebyshev nodes of [-1/2, 1/2] (relative error
+// 2e-14), n added to the exponent field.  Adding 1.5 2^52 leaves n in the sum's low word: no conversion and no ldexp.  Below -1000 (and -inf): 0
 __device__ __forceinline__ double pow2_64(double x) {
-  x = fmax(x, -1100.0);
-  const double n = rint(x), f = x - n;
-  constexpr double L = 0.693147180559945309417;
-  constexpr double L2 = L * L, L3 = L2 * L, L4 = L2 * L2, L5 = L4 * L, L6 = L3 * L3, L7 = L6 * L, L8 = L4 * L4, L9 = L8 * L, L10 = L5 * L5, L11 = L10 * L;
-  double p = L11 / 39916800.0;
-  p = fma(p, f, L10 / 3628800.0);
-  p = fma(p, f, L9 / 362880.0);
-  p = fma(p, f, L8 / 40320.0);
-  p = fma(p, f, L7 / 5040.0);
-  p = fma(p, f, L6 / 720.0);
-  p = fma(p, f, L5 / 120.0);
-  p = fma(p, f, L4 / 24.0);
-  p = fma(p, f, L3 / 6.0);
-  p = fma(p, f, L2 / 2.0);
-  p = fma(p, f, L);
-  p = fma(p, f, 1.0);
-  return ldexp(p, (int)n);
+  constexpr double MAGIC = 6755399441055744.0;
+  const double y = x + MAGIC, f = x - (y - MAGIC);
+  double p = 1.02059054137655955e-07;
+  p = fma(p, f, 1.32596452448871106e-06);
+  p = fma(p, f, 1.52526729248507372e-05);
+  p = fma(p, f, 1.54034337512510097e-04);
+  p = fma(p, f, 1.33335582007945925e-03);
+  p = fma(p, f, 9.61812919393431262e-03);
+  p = fma(p, f, 5.55041086646516704e-02);
+  p = fma(p, f, 2.40226506956403407e-01);
+  p = fma(p, f, 6.93147180559946174e-01);
+  p = fma(p, f, 1.00000000000001354e+00);
+  const double r = __hiloint2double(__double2hiint(p) + (__double2loint(y) << 20), __double2loint(p));
+  return x > -1000.0 ? r : 0.0;
 }
 // weight of logit l under the maximum m, c = log2(e) / tau: 2^(c l - c m); an infinite maximum shares the mass among its equals
 struct Weigh {
@@ -159,6 +156,16 @@ __global__ __launch_bounds__(VT) void verify_accept_kernel(VerifyArgs a) {
   const int piece = blockIdx.x, b = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int n = drafted(a, b);
+  // what lane i of wave 0 needs to judge draft i, requested before the rows' statistics
+  float u = 0.f, lx = 0.f, qx = 0.f;
+  long long x = -1;
+  if (tid < n) {
+    x = a.tokens[(long)b * a.K + tid];
+    u = a.u[(long)b * a.K + tid];
+    const long long xc = min(max(x, 0LL), (long long)a.V - 1);
+    lx = logit<T>((const T*)a.target + a.t_sb * b + a.t_sr * tid, xc);
+    if (a.draft) qx = logit<T>((const T*)a.draft + a.d_sb * b + a.d_sr * tid, xc);
+  }
   // rows 0..n of the target, then n of the draft: sixteen lanes each
   const int nrows = a.draft ? 2 * n + 1 : n + 1;
   for (int q = tid >> 4; q < nrows; q += VT / 16) {
@@ -178,16 +185,10 @@ __global__ __launch_bounds__(VT) void verify_accept_kernel(VerifyArgs a) {
   __syncthreads();
   if (wave == 0) {                                                    // lane i judges draft i
     bool ok = false;
-    if (lane < n) {
-      const long long x = a.tokens[(long)b * a.K + lane];
-      if (x >= 0 && x < a.V) {
-        const float u = a.u[(long)b * a.K + lane];
-        const float lp = logit<T>((const T*)a.target + a.t_sb * b + a.t_sr * lane, x);
-        const float lq = a.draft ? logit<T>((const T*)a.draft + a.d_sb * b + a.d_sr * lane, x) : 0.f;
-        const double p = Weigh(row_m[lane], a.c)(lp) / row_s[lane];
-        const double q = a.draft ? Weigh(row_m[n + 1 + lane], a.c)(lq) / row_s[n + 1 + lane] : 1.0;
-        ok = (double)u * q < p;
-      }
+    if (lane < n && x >= 0 && x < a.V) {
+      const double p = Weigh(row_m[lane], a.c)(lx) / row_s[lane];
+      const double q = a.draft ? Weigh(row_m[n + 1 + lane], a.c)(qx) / row_s[n + 1 + lane] : 1.0;
+      ok = (double)u * q < p;
     }
     const unsigned long long bad = ~__builtin_amdgcn_ballot_w64(ok);
     const int kept = min(n, (int)__builtin_ctzll(bad | (1ull << 63)));
@@ -337,6 +338,7 @@ __global__ __launch_bounds__(VT) void verify_sample_kernel(VerifyArgs a) {
   if (tid == 0) { s_at = 0x7fffffff; s_last = -1; }
   __syncthreads();
   double sum = 0.0;
+#pragma unroll
   for (int e = 0; e < VE; ++e) sum += f[tid * (VE + 1) + e];
   const double incl = wave_scan64(sum, lane);
   if (lane == 63) wsum[wave] = incl;
@@ -345,6 +347,7 @@ __global__ __launch_bounds__(VT) void verify_sample_kernel(VerifyArgs a) {
   for (int i = 0; i < wave; ++i) run += wsum[i];
   const int c0 = piece * PIECE + tid * VE;
   int at = 0x7fffffff, last = -1;
+#pragma unroll
   for (int e = 0; e < VE; ++e) {
     const double x = f[tid * (VE + 1) + e];
     run += x;
