@@ -391,7 +391,7 @@ int neko_kv8_append(void* k8, void* v8, float* k_scale, float* v_scale, int dtyp
                     long k_ss, long k_st, const uint16_t* v, long v_ss, long v_st, const int* pos, const int* n_new, int T, void* stream);
 int neko_kv8_read(const void* k8, const void* v8, const float* k_scale, const float* v_scale, int dtype, int nseq, int H, int cap, int hd,
                   int block, const int* length, int L, uint16_t* k, uint16_t* v, void* stream);
-long neko_attn_kv8_ws_floats(int nseq, int H, int G, int cap, int hd, int T, int max_len);
+long neko_attn_kv8_ws_floats(int nseq, int H, int G, int cap, int hd, int T, int window, int sinks, int max_len);
 int neko_attn_kv8(const void* k8, const void* v8, const float* k_scale, const float* v_scale, int dtype, int nseq, int H, int cap, int hd, int block,
                   const uint16_t* q, long q_ss, long q_st, uint16_t* out, long o_ss, long o_st, int G, int T, const int* pos, const int* n_new,
                   const int* start, int window, int sinks, float scale, int max_len, float* ws, long ws_floats, void* stream);

@@ -71,7 +71,7 @@ SIGNATURES = {
     "neko_patch_pos_add_bwd": [_vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
     "neko_kv8_append": [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _l, _l, _vp, _l, _l, _vp, _vp, _i, _vp],
     "neko_kv8_read": [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _i, _vp, _vp, _vp],
-    "neko_attn_kv8_ws_floats": [_i, _i, _i, _i, _i, _i, _i],
+    "neko_attn_kv8_ws_floats": [_i, _i, _i, _i, _i, _i, _i, _i, _i],
     "neko_attn_kv8": [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _l, _l, _vp, _l, _l, _i, _i, _vp, _vp, _vp, _i, _i, _f, _i, _vp, _l, _vp],
     "neko_verify_draft_ws_bytes": [_i, _i, _i],
     "neko_verify_draft": [_vp, _l, _l, _vp, _l, _l, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _f, _vp, _vp, _vp, _l, _vp],

@@ -70,7 +70,7 @@ __device__ __forceinline__ bool visible(const AttnArgs& a, const Span& sp, int k
 constexpr int KT = 64;
 
 template <int HD, int DT, int NQ, int NW>
-__global__ __launch_bounds__(NW * 64) void attn_kv8_rows_kernel(AttnArgs a) {
+__global__ __launch_bounds__(NW * 64, NQ == 1 || (NQ == 2 && HD < 128) ? 2 : 1) void attn_kv8_rows_kernel(AttnArgs a) {
   constexpr int NC = HD / 16;                 // channel tiles
   constexpr int NK = HD / 32;                 // contraction steps of the scores
   constexpr int LDO = HD + 4;
@@ -538,9 +538,10 @@ __global__ __launch_bounds__(256) void attn_kv8_merge_kernel(AttnArgs a, int row
 }
 
 // How a call is cut.  More than 64 rows a key head go through LDS tiles (a row tile of 128 or 256); up to 64 stay in the register kernel, 16 / 32 /
-// 64 rows a wave.  The key axis is split until the grid fills the chip.
+// 64 rows a wave.  The key axis is cut into the number of splits with the least estimated time: rounds of resident workgroups x (64-key tiles of
+// the longest wave + a constant for start and end) + the merge of the partial results.  `keys`: the most a row can see.
 struct Plan { int tiled, nq, nw, rt, rtiles, splits; };
-Plan plan_of(int S, int H, int hd, int rows, int max_len) {
+Plan plan_of(int S, int H, int hd, int rows, int keys) {
   Plan p;
   p.tiled = rows > 64;
   if (p.tiled) {
@@ -554,14 +555,25 @@ Plan plan_of(int S, int H, int hd, int rows, int max_len) {
   }
   p.rtiles = (rows + p.rt - 1) / p.rt;
   const long base = (long)S * H * p.rtiles;
-  const long tiles = (max_len + KT - 1) / KT;
-  const long want = p.tiled ? 256 : 1024;              // workgroups
-  long sp = (want + base - 1) / base;
-  const long most = p.tiled ? (tiles + 7) / 8 : (tiles + p.nw - 1) / p.nw;      // 8 tiles a workgroup | a tile a wave
-  if (p.tiled && base * 4 > 3 * want) sp = 1;          // three quarters full: a second pass over the partial sums costs more
-  p.splits = (int)(sp < 1 ? 1 : sp < most ? sp : most);
-  if (p.splits < 1) p.splits = 1;
+  const int tiles = (keys + KT - 1) / KT;
+  const int per_wg = p.tiled ? 1 : p.nw;               // key tiles a workgroup works on at a time
+  const long slots = 256L * (p.tiled ? (hd == 128 ? 1 : 2) : p.nq == 1 ? (hd == 128 ? 1 : 2) : (p.nq == 2 && hd < 128 ? 2 : 1));
+  const int fixed = p.tiled ? 4 : 2;
+  int best = 1;
+  double best_t = 0;
+  for (int sp = 1; sp <= 64 && (sp == 1 || (sp - 1) * per_wg < tiles); ++sp) {
+    const long rounds = (base * sp + slots - 1) / slots;
+    const int per = (tiles + sp - 1) / sp;
+    const double t = (double)rounds * ((per + per_wg - 1) / per_wg + fixed) + (sp > 1 ? 2.0 + 0.1 * sp : 0.0);
+    if (sp == 1 || t < best_t * 0.97) { best = sp; best_t = t; }
+  }
+  p.splits = best;
   return p;
+}
+int keys_of(int cap, int T, int window, int sinks, int max_len) {
+  long k = max_len > 0 && max_len < cap ? max_len : cap;
+  if (window > 0 && (long)window + sinks + T + KT < k) k = (long)window + sinks + T + KT;
+  return (int)k;
 }
 
 template <int HD, int DT>
@@ -583,9 +595,9 @@ int launch_rows(const AttnArgs& a, const Plan& p, hipStream_t s) {
 
 }  // namespace
 
-long neko_attn_kv8_ws_floats_impl(int S, int H, int G, int cap, int hd, int T, int max_len) {
+long neko_attn_kv8_ws_floats_impl(int S, int H, int G, int cap, int hd, int T, int window, int sinks, int max_len) {
   if (S <= 0 || H <= 0 || G <= 0 || T <= 0 || cap <= 0 || hd <= 0) return 0;
-  const Plan p = plan_of(S, H, hd, T * G, max_len > 0 && max_len < cap ? max_len : cap);
+  const Plan p = plan_of(S, H, hd, T * G, keys_of(cap, T, window, sinks, max_len));
   return p.splits > 1 ? (long)S * H * p.splits * p.rtiles * p.rt * (hd + 2) : 0;
 }
 
@@ -597,9 +609,8 @@ int neko_attn_kv8_impl(const uint8_t* k8, const uint8_t* v8, const float* ks, co
   if (rc) return rc;
   if (T > cap || (long)T * G > (1 << 24)) return NEKO_ERR_ARG;
   if (((uintptr_t)q | (uintptr_t)out) & 15 || (q_ss | q_st | o_ss | o_st) & 7) return NEKO_ERR_ARG;
-  if (max_len <= 0 || max_len > cap) max_len = cap;
-  const Plan p = plan_of(S, H, hd, T * G, max_len);
-  const long need = neko_attn_kv8_ws_floats_impl(S, H, G, cap, hd, T, max_len);
+  const Plan p = plan_of(S, H, hd, T * G, keys_of(cap, T, window, sinks, max_len));
+  const long need = p.splits > 1 ? (long)S * H * p.splits * p.rtiles * p.rt * (hd + 2) : 0;
   if (need > ws_floats || (need && !ws)) return NEKO_ERR_ARG;
   const int bshift = block == 16 ? 4 : block == 32 ? 5 : 6;
   AttnArgs a{k8, v8, ks, vs, q, out, q_ss, q_st, o_ss, o_st, pos, n_new, start, ws, nullptr, S, H, G, cap, T, bshift, window, sinks, p.splits, p.rtiles,

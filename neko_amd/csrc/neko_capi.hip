@@ -275,8 +275,8 @@ int neko_kv8_read(const void* k8, const void* v8, const float* k_scale, const fl
   return neko_kv8_read_impl(static_cast<const uint8_t*>(k8), static_cast<const uint8_t*>(v8), k_scale, v_scale, dtype, nseq, H, cap, hd, block, length,
                             L, k, v, S(stream));
 }
-long neko_attn_kv8_ws_floats(int nseq, int H, int G, int cap, int hd, int T, int max_len) {
-  return neko_attn_kv8_ws_floats_impl(nseq, H, G, cap, hd, T, max_len);
+long neko_attn_kv8_ws_floats(int nseq, int H, int G, int cap, int hd, int T, int window, int sinks, int max_len) {
+  return neko_attn_kv8_ws_floats_impl(nseq, H, G, cap, hd, T, window, sinks, max_len);
 }
 int neko_attn_kv8(const void* k8, const void* v8, const float* k_scale, const float* v_scale, int dtype, int nseq, int H, int cap, int hd, int block,
                   const uint16_t* q, long q_ss, long q_st, uint16_t* out, long o_ss, long o_st, int G, int T, const int* pos, const int* n_new,

@@ -161,7 +161,7 @@ int neko_kv8_append_impl(uint8_t* k8, uint8_t* v8, float* ks, float* vs, int dty
                          long k_st, const bf16_t* v, long v_ss, long v_st, const int* pos, const int* n_new, int T, hipStream_t s);
 int neko_kv8_read_impl(const uint8_t* k8, const uint8_t* v8, const float* ks, const float* vs, int dtype, int S, int H, int cap, int hd, int block,
                        const int* length, int L, bf16_t* k, bf16_t* v, hipStream_t s);
-long neko_attn_kv8_ws_floats_impl(int S, int H, int G, int cap, int hd, int T, int max_len);
+long neko_attn_kv8_ws_floats_impl(int S, int H, int G, int cap, int hd, int T, int window, int sinks, int max_len);
 int neko_attn_kv8_impl(const uint8_t* k8, const uint8_t* v8, const float* ks, const float* vs, int dtype, int S, int H, int cap, int hd, int block,
                        const bf16_t* q, long q_ss, long q_st, bf16_t* out, long o_ss, long o_st, int G, int T, const int* pos, const int* n_new,
                        const int* start, int window, int sinks, float scale, int max_len, float* ws, long ws_floats, hipStream_t s);

@@ -41,9 +41,13 @@ template <typename T> __device__ __forceinline__ float logit(const T* p, long i)
 template <> __device__ __forceinline__ float logit<float>(const float* p, long i) { const float x = p[i]; return x == x ? x : -INFINITY; }
 template <> __device__ __forceinline__ float logit<bf16_t>(const bf16_t* p, long i) { const float x = bf16_to_f32(p[i]); return x == x ? x : -INFINITY; }
 
+template <typename T> __device__ __forceinline__ float raw_logit(const T* p, int i);
+template <> __device__ __forceinline__ float raw_logit<float>(const float* p, int i) { return p[i]; }
+template <> __device__ __forceinline__ float raw_logit<bf16_t>(const bf16_t* p, int i) { return bf16_to_f32(p[i]); }
+
 // 2^x for x <= 1/2, fp64: x = n + f, the polynomial of degree 9 that interpolates 2^f at the ten Chebyshev nodes of [-1/2, 1/2] (relative error
-// 2e-14), n added to the exponent field.  Adding 1.5 2^52 leaves n in the sum's low word: no conversion and no ldexp.  Below -1000 (and -inf): 0
-__device__ __forceinline__ double pow2_64(double x) {
+// 2e-14), n added to the exponent field.  Adding 1.5 2^52 leaves n in the sum's low word: no conversion and no ldexp.  pow2_64: 0 below -1000, for -inf and for NaN
+__device__ __forceinline__ double pow2_64_above_1000(double x) {
   constexpr double MAGIC = 6755399441055744.0;
   const double y = x + MAGIC, f = x - (y - MAGIC);
   double p = 1.02059054137655955e-07;
@@ -56,7 +60,10 @@ __device__ __forceinline__ double pow2_64(double x) {
   p = fma(p, f, 2.40226506956403407e-01);
   p = fma(p, f, 6.93147180559946174e-01);
   p = fma(p, f, 1.00000000000001354e+00);
-  const double r = __hiloint2double(__double2hiint(p) + (__double2loint(y) << 20), __double2loint(p));
+  return __hiloint2double(__double2hiint(p) + (__double2loint(y) << 20), __double2loint(p));
+}
+__device__ __forceinline__ double pow2_64(double x) {
+  const double r = pow2_64_above_1000(x);
   return x > -1000.0 ? r : 0.0;
 }
 // weight of logit l under the maximum m, c = log2(e) / tau: 2^(c l - c m); an infinite maximum shares the mass among its equals
@@ -66,7 +73,7 @@ struct Weigh {
   bool inf;
   __device__ __forceinline__ Weigh(float m_, double c_) : c(c_), cm((double)m_ * c_), m(m_), inf(m_ == INFINITY || m_ == -INFINITY) {}
   __device__ __forceinline__ double operator()(float l) const {
-    if (inf) return l == m && m == INFINITY ? 1.0 : 0.0;
+    if (__builtin_expect(inf, 0)) return l == m && m == INFINITY ? 1.0 : 0.0;
     return pow2_64(fma((double)l, c, -cm));
   }
 };
@@ -86,7 +93,9 @@ __device__ __forceinline__ double wave_scan64(double v, int lane) {       // inc
 __device__ __forceinline__ int drafted(const VerifyArgs& a, int b) { return min(max(a.n_draft ? a.n_draft[b] : a.K, 0), a.K); }
 
 // ---- launch 1: every row piece -> maximum and sum (or the maximum's index) ----
-template <typename T>
+// Bound by the vector unit: an element costs 20 instructions (15 of them fp64), so everything else stays out of the loop: whole pieces load and
+// compare without bounds, and a NaN needs no test (the maximum ignores it, the lower bound of the exponent turns it into nothing).
+template <typename T, bool GREEDY>
 __global__ __launch_bounds__(VT) void verify_rows_kernel(VerifyArgs a) {
   __shared__ float sm[VT / 64];
   __shared__ double ss[VT / 64];
@@ -96,43 +105,60 @@ __global__ __launch_bounds__(VT) void verify_rows_kernel(VerifyArgs a) {
   const bool is_draft = row > a.K;
   const int i = is_draft ? row - a.K - 1 : row;
   if (is_draft ? i >= n : i > n) return;                              // rows behind the drafted ones are not looked at
-  const T* z = is_draft ? (const T*)a.draft + a.d_sb * b + a.d_sr * i : (const T*)a.target + a.t_sb * b + a.t_sr * i;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tid = threadIdx.x;
   const int c0 = piece * PIECE;
+  const T* z = (is_draft ? (const T*)a.draft + a.d_sb * b + a.d_sr * i : (const T*)a.target + a.t_sb * b + a.t_sr * i) + c0;
+  const int left = a.V - c0;                                          // columns of this piece
   float x[VE];
+  if (left >= PIECE) {
 #pragma unroll
-  for (int e = 0; e < VE; ++e) {
-    const int c = c0 + e * VT + threadIdx.x;
-    x[e] = logit<T>(z, min(c, a.V - 1));
-    if (c >= a.V) x[e] = -INFINITY;
+    for (int e = 0; e < VE; ++e) x[e] = raw_logit<T>(z + e * VT, tid);
+  } else {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      const int c = e * VT + tid;
+      x[e] = raw_logit<T>(z, min(c, left - 1));
+      if (c >= left) x[e] = -INFINITY;
+    }
   }
-  float m = x[0];
-  int at = c0 + (int)threadIdx.x;
+  float m = x[0] == x[0] ? x[0] : -INFINITY;
+  int at = tid;
 #pragma unroll
-  for (int e = 1; e < VE; ++e)
-    if (x[e] > m) { m = x[e]; at = c0 + e * VT + (int)threadIdx.x; }
-  float wm = wave_max(m);
+  for (int e = 1; e < VE; ++e) {
+    if (GREEDY) {
+      if (x[e] > m) { m = x[e]; at = e * VT + tid; }
+    } else {
+      m = fmaxf(m, x[e]);
+    }
+  }
+  const float wm = wave_max(m);
   if (lane == 0) sm[wave] = wm;
   __syncthreads();
-  const float bm = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+  const float bm = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3])))));
   const long o = ((long)b * (2 * a.K + 1) + row) * a.pieces + piece;
-  if (a.greedy) {
+  if (GREEDY) {
     int idx = m == bm ? at : 0x7fffffff;                              // lowest index among equals
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) idx = min(idx, __shfl_xor(idx, d, 64));
     if (lane == 0) si[wave] = idx;
     __syncthreads();
-    if (threadIdx.x == 0) { a.pm[o] = bm; a.ps[o] = (double)min(min(si[0], si[1]), min(si[2], si[3])); }
+    if (tid == 0) { a.pm[o] = bm; a.ps[o] = (double)(c0 + min(min(si[0], si[1]), min(si[2], si[3]))); }
     return;
   }
-  const Weigh w(bm, a.c);
   double s = 0.0;
+  if (bm == INFINITY || bm == -INFINITY) {
 #pragma unroll
-  for (int e = 0; e < VE; ++e) s += w(x[e]);
+    for (int e = 0; e < VE; ++e) s += x[e] == bm && bm == INFINITY ? 1.0 : 0.0;
+  } else {
+    const double cm = (double)bm * a.c;
+    // exponents stop at -1000: 2^-1000 beside the 1 of the maximum is nothing, and the exponent field does not run over
+#pragma unroll
+    for (int e = 0; e < VE; ++e) s += pow2_64_above_1000(fmax(fma((double)x[e], a.c, -cm), -1000.0));
+  }
   s = wave_sum64(s);
   if (lane == 0) ss[wave] = s;
   __syncthreads();
-  if (threadIdx.x == 0) { a.pm[o] = bm; a.ps[o] = (ss[0] + ss[1]) + (ss[2] + ss[3]); }
+  if (tid == 0) { a.pm[o] = bm; a.ps[o] = (ss[0] + ss[1]) + (ss[2] + ss[3]); }
 }
 
 // What is sampled from once `kept` are kept: target row and maximum and 1 / sum, and the draft row's that is taken off (or one token).
@@ -365,7 +391,8 @@ __global__ __launch_bounds__(VT) void verify_sample_kernel(VerifyArgs a) {
 template <typename T>
 int launch(const VerifyArgs& a, hipStream_t s) {
   const int rows = a.greedy || !a.draft ? a.K + 1 : 2 * a.K + 1;
-  hipLaunchKernelGGL((verify_rows_kernel<T>), dim3(a.pieces, rows, a.B), dim3(VT), 0, s, a);
+  if (a.greedy) hipLaunchKernelGGL((verify_rows_kernel<T, true>), dim3(a.pieces, rows, a.B), dim3(VT), 0, s, a);
+  else hipLaunchKernelGGL((verify_rows_kernel<T, false>), dim3(a.pieces, rows, a.B), dim3(VT), 0, s, a);
   NEKO_CHECK_LAUNCH();
   if (a.greedy) {
     hipLaunchKernelGGL(verify_greedy_kernel, dim3(a.B), dim3(VT), 0, s, a);

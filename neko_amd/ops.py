@@ -725,7 +725,7 @@ def attn_kv8(cache: KV8Cache, q: torch.Tensor, pos: torch.Tensor, n_new: Optiona
     assert To == T, "out must have q's rows"
     lib = _lib.load()
     G = HG // cache.heads
-    nws = lib.neko_attn_kv8_ws_floats(cache.nseq, cache.heads, G, cache.cap, cache.hd, T, int(max_len))
+    nws = lib.neko_attn_kv8_ws_floats(cache.nseq, cache.heads, G, cache.cap, cache.hd, T, int(window), int(sinks), int(max_len))
     ws = torch.empty(nws, dtype=torch.float32, device=cache.device) if nws else None
     _lib.call("neko_attn_kv8", *cache._args, q.data_ptr(), q_ss, q_st, out.data_ptr(), o_ss, o_st, G, T, pos.data_ptr(), _p(n_new), _p(start),
               int(window), int(sinks), float(scale) if scale is not None else cache.hd ** -0.5, int(max_len), _p(ws), nws, _stream())

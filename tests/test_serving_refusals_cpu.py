@@ -56,8 +56,9 @@ def test_distill_refuses(bad):
 
 def test_workspace_sizes():
     lib = _lib.load()
-    assert lib.neko_attn_kv8_ws_floats(0, 1, 1, 64, 32, 1, 0) == 0 and lib.neko_attn_kv8_ws_floats(64, 24, 1, 64, 32, 1, 0) == 0
-    assert lib.neko_attn_kv8_ws_floats(1, 1, 1, 8192, 128, 1, 0) > 0 and lib.neko_attn_kv8_ws_floats(1, 1, 1, 8192, 128, 1, 64) == 0
+    assert lib.neko_attn_kv8_ws_floats(0, 1, 1, 64, 32, 1, 0, 0, 0) == 0 and lib.neko_attn_kv8_ws_floats(64, 24, 1, 64, 32, 1, 0, 0, 0) == 0
+    assert lib.neko_attn_kv8_ws_floats(1, 1, 1, 8192, 128, 1, 0, 0, 0) > 0 and lib.neko_attn_kv8_ws_floats(1, 1, 1, 8192, 128, 1, 0, 0, 64) == 0
+    assert lib.neko_attn_kv8_ws_floats(1, 1, 1, 8192, 128, 1, 50, 4, 0) == 0
     assert lib.neko_verify_draft_ws_bytes(0, 1, 1) == 0 and lib.neko_verify_draft_ws_bytes(2, 3, 5000) > 0
 
 
