@@ -10,9 +10,11 @@
 // that could spread beyond its own position.
 //
 // Both kernels are bound by HBM: append reads 2 B and writes 1 B a value, the read back 1 B and 2 B.  A lane owns 16 positions x 8
-// channels: 16 row loads of 16 B in flight before the first is looked at, the block's maximum meets in registers (shuffles inside the
-// wave, no LDS), and V's transposed tile leaves as eight whole 16-byte pieces that no other lane touches -- so a partly filled tile is
-// read, changed and written by its one owner.  Consecutive units of a wave are consecutive heads: their row pieces are adjacent.
+// channels: 16 row loads of 16 B in flight before the first is looked at, and the block's maximum meets in registers (shuffles inside the
+// wave).  Consecutive units of a wave are consecutive heads: their row pieces are adjacent in the bf16 rows.  On the 8-bit side a head's
+// bytes are contiguous instead, so the codes change hands through LDS: written and read there in the lane's own order, moved to and from
+// memory as consecutive 16-byte pieces (as 8-byte rows and 16-byte pieces 128 B apart they were 3 x the requests).  A piece belongs to
+// one lane: a partly filled one is read, changed and written by its owner.
 #include "kv8.h"
 
 namespace {
@@ -49,9 +51,16 @@ __device__ __forceinline__ uint32_t pkmax_u16(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
 }
 
+// a unit (one block of one head, K or V) on its way out: where it goes, its first position, the new positions [pc, end) (end < 0: nothing),
+// and the factor of its older codes if their grid grew (0: it did not)
+struct UnitOut { long base; int b0, pc, end; float ratio; };
+
 template <int HD, int BLOCK, int DT>
 __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
   constexpr int C = HD / 8, R = BLOCK / 16, U = 64 / (C * R);      // channel lanes, tile lanes, units per wave
+  constexpr int UB = BLOCK * HD, US = UB + 32;                      // bytes of a unit, and its stride in the image (8 units: all banks)
+  __shared__ __attribute__((aligned(16))) char img[4][U * US];
+  __shared__ UnitOut outs[4][U];
   const bool is_v = blockIdx.y != 0;
   const int lane = threadIdx.x & 63;
   const int c = lane % C, ui = (lane / C) % U, r = lane / (C * U);
@@ -104,89 +113,97 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
   for (int o = 1; o < C; o <<= 1) am = max(am, (uint32_t)__shfl_xor((int)am, o, 64));
 #pragma unroll
   for (int o = C * U; o < 64; o <<= 1) am = max(am, (uint32_t)__shfl_xor((int)am, o, 64));
-  if (!act) return;
-
   // bf16 bits -> exponent of the scale: am = (1 + m / 128) 2^(x - 127); qmax = 1.75 * 2^8 | (1 + 126 / 128) * 2^6
   const int x = (int)(am >> 7), m = (int)(am & 0x7f);
   int e = DT == 0 ? x - 127 - 8 + (m > 96) : x - 127 - 6 + (m > 126);
   if (x == 0 || e < -100) e = -100;
   float scale = __uint_as_float((uint32_t)(e + 127) << 23);
-  float* sp = (is_v ? a.vs : a.ks) + ((long)s * a.H + h) * (a.cap >> a.bshift) + blk;
-  const bool held = b0 < pc;                                        // the block holds older rows
+  const long head = (long)s * a.H + h;
+  float* sp = (is_v ? a.vs : a.ks) + head * (a.cap >> a.bshift) + blk;
+  const bool held = act && b0 < pc;                                 // the block holds older rows
   const float was = held ? *sp : scale;
   scale = fmaxf(scale, was);
   const bool grew = held && scale > was;
-  if (c == 0 && r == 0) *sp = scale;      // (every lane of the unit is in this wave and has read it: the loads stand before the store)
-  const float inv = 1.0f / scale, ratio = was * inv;
-  const long head = ((long)s * a.H + h);
-  if (!any_new && !grew) return;
-
-  if (!is_v) {
-    uint8_t* kp = a.k8 + (head * a.cap + t0) * HD + c * 8;
+  const float inv = 1.0f / scale;
+  if (c == 0 && r == 0) {                 // (every lane of the unit is in this wave and has read the old scale: the loads stand before the store)
+    if (act) *sp = scale;
+    UnitOut& o = outs[threadIdx.x >> 6][ui];
+    o.base = (head * a.cap + b0) * HD;    // K and V alike: a block's bytes are contiguous in both layouts
+    o.b0 = b0;
+    o.pc = pc;
+    o.end = act ? end : -1;
+    o.ratio = grew ? was * inv : 0.f;
+  }
+  // codes -> the wave's image of its units, as they will lie in memory (bytes of positions that are not new: whatever they are, dropped below)
+  char* mine = img[threadIdx.x >> 6];
+  if (any_new) {
+    char* at = mine + ui * US + r * (16 * HD);
+    if (!is_v) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int t = t0 + i;
-      if (t >= pc && t < end) {
+      for (int i = 0; i < 16; ++i) {
         uint2 w;
         w.x = kv8_pack4<DT>(lo_f(raw[i].x) * inv, hi_f(raw[i].x) * inv, lo_f(raw[i].y) * inv, hi_f(raw[i].y) * inv);
         w.y = kv8_pack4<DT>(lo_f(raw[i].z) * inv, hi_f(raw[i].z) * inv, lo_f(raw[i].w) * inv, hi_f(raw[i].w) * inv);
-        *reinterpret_cast<uint2*>(kp + (long)i * HD) = w;
+        *reinterpret_cast<uint2*>(at + i * HD + c * 8) = w;
       }
-    }
-    if (grew) {
-      for (int i = 0; i < 16 && t0 + i < pc; ++i) {
-        uint2 w = *reinterpret_cast<const uint2*>(kp + (long)i * HD);
-        uint32_t q[2] = {w.x, w.y};
+    } else {
 #pragma unroll
-        for (int d = 0; d < 2; ++d)
-          q[d] = kv8_pack4<DT>(kv8_code<DT>(q[d] & 0xff) * ratio, kv8_code<DT>((q[d] >> 8) & 0xff) * ratio, kv8_code<DT>((q[d] >> 16) & 0xff) * ratio,
-                               kv8_code<DT>(q[d] >> 24) * ratio);
-        *reinterpret_cast<uint2*>(kp + (long)i * HD) = make_uint2(q[0], q[1]);
+      for (int ch = 0; ch < 8; ++ch) {
+        uint32_t q[4];
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          float f[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint4& w4 = raw[d * 4 + i];
+            const uint32_t w = ch < 2 ? w4.x : ch < 4 ? w4.y : ch < 6 ? w4.z : w4.w;
+            f[i] = ((ch & 1) ? hi_f(w) : lo_f(w)) * inv;
+          }
+          q[d] = kv8_pack4<DT>(f[0], f[1], f[2], f[3]);
+        }
+        *reinterpret_cast<uint4*>(at + (c * 8 + ch) * 16) = make_uint4(q[0], q[1], q[2], q[3]);
       }
     }
-    return;
   }
-  // V: eight channels of one transposed tile, 16 bytes each
-  uint8_t* vp = a.v8 + (head * (a.cap >> 4) + (t0 >> 4)) * (HD * 16) + c * 128;
-  const int i0 = max(pc - t0, 0), i1 = min(end - t0, 16);           // new positions of the tile: [i0, i1)
-  const bool whole = i0 == 0 && i1 == 16;
-#pragma unroll
-  for (int ch = 0; ch < 8; ++ch) {
-    uint32_t q[4] = {0, 0, 0, 0};
-    if (any_new) {
-#pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        float f[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint4& w4 = raw[d * 4 + i];
-          const uint32_t w = ch < 2 ? w4.x : ch < 4 ? w4.y : ch < 6 ? w4.z : w4.w;
-          f[i] = ((ch & 1) ? hi_f(w) : lo_f(w)) * inv;
-        }
-        q[d] = kv8_pack4<DT>(f[0], f[1], f[2], f[3]);
-      }
-    }
-    if (!whole) {
-      const uint4 o4 = *reinterpret_cast<const uint4*>(vp + ch * 16);
-      uint32_t o[4] = {o4.x, o4.y, o4.z, o4.w};
+  __syncthreads();
+  // the image leaves in whole 16-byte pieces, consecutive lanes consecutive pieces; K: a piece of one row, V: sixteen positions of one channel
+  uint8_t* out = is_v ? a.v8 : a.k8;
+#pragma unroll 2
+  for (int it = 0; it < 8; ++it) {
+    const int p16 = it * 64 + lane;
+    const int u2 = p16 / (UB / 16), off = (p16 % (UB / 16)) * 16;
+    const UnitOut o = outs[threadIdx.x >> 6][u2];
+    // positions of the piece: [t, t + len); new ones among them: [i0, i1)
+    const int t = o.b0 + (is_v ? off / (16 * HD) * 16 : off / HD), len = is_v ? 16 : 1;
+    const int i0 = max(o.pc - t, 0), i1 = min(o.end - t, len);
+    const bool old = o.ratio != 0.f && t < o.pc;                    // older positions whose grid grew
+    if (o.end < 0 || (i0 >= i1 && !old)) continue;
+    const uint4 w = *reinterpret_cast<const uint4*>(mine + u2 * US + off);
+    uint32_t q[4] = {w.x, w.y, w.z, w.w};
+    uint4* dst = reinterpret_cast<uint4*>(out + o.base + off);
+    if (i0 > 0 || i1 < len) {                                       // partly new: this lane owns the piece, so it may change it in place
+      const uint4 g = *dst;
+      uint32_t k[4] = {g.x, g.y, g.z, g.w};
 #pragma unroll
       for (int d = 0; d < 4; ++d) {
-        uint32_t keep = 0, old = 0;                                 // bytes that stay (as they are, or on the grown grid)
+        uint32_t keep = 0xffffffffu, was_old = 0xffffffffu;
+        if (is_v) {
+          keep = was_old = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int t = d * 4 + i;
-          if (t < i0 || t >= i1) keep |= 0xffu << (8 * i);
-          if (t0 + t < pc) old |= 0xffu << (8 * i);
+          for (int i = 0; i < 4; ++i) {
+            if (4 * d + i < i0 || 4 * d + i >= i1) keep |= 0xffu << (8 * i);
+            if (t + 4 * d + i < o.pc) was_old |= 0xffu << (8 * i);
+          }
         }
-        if (grew && old) {
-          const uint32_t re = kv8_pack4<DT>(kv8_code<DT>(o[d] & 0xff) * ratio, kv8_code<DT>((o[d] >> 8) & 0xff) * ratio,
-                                            kv8_code<DT>((o[d] >> 16) & 0xff) * ratio, kv8_code<DT>(o[d] >> 24) * ratio);
-          o[d] = (re & old) | (o[d] & ~old);
+        if (old) {
+          const uint32_t re = kv8_pack4<DT>(kv8_code<DT>(k[d] & 0xff) * o.ratio, kv8_code<DT>((k[d] >> 8) & 0xff) * o.ratio,
+                                            kv8_code<DT>((k[d] >> 16) & 0xff) * o.ratio, kv8_code<DT>(k[d] >> 24) * o.ratio);
+          k[d] = (re & was_old) | (k[d] & ~was_old);
         }
-        q[d] = (o[d] & keep) | (q[d] & ~keep);
+        q[d] = (k[d] & keep) | (q[d] & ~keep);
       }
     }
-    *reinterpret_cast<uint4*>(vp + ch * 16) = make_uint4(q[0], q[1], q[2], q[3]);
+    *dst = make_uint4(q[0], q[1], q[2], q[3]);
   }
 }
 
@@ -201,45 +218,56 @@ struct ReadArgs {
 
 template <int HD, int DT>
 __global__ __launch_bounds__(256) void kv8_read_kernel(ReadArgs a) {
-  constexpr int C = HD / 8;
+  constexpr int C = HD / 8, U = 64 / C;                             // lanes and units (16 positions of a head) of a wave
+  constexpr int UB = 16 * HD, US = UB + 32;
+  __shared__ __attribute__((aligned(16))) char img[4][U * US];
   const bool is_v = blockIdx.y != 0;
-  const long id = (long)blockIdx.x * 256 + threadIdx.x;
-  const int c = (int)(id % C);
-  const long u = id / C;
-  if (u >= a.units) return;
-  const int h = (int)(u % a.H);
-  const long sj = u / a.H;
+  const int lane = threadIdx.x & 63;
+  const int c = lane % C, ui = lane / C;
+  const long u = ((long)blockIdx.x * 4 + (threadIdx.x >> 6)) * U + ui;
+  const bool act = u < a.units;
+  const long uu = act ? u : a.units - 1;
+  const int h = (int)(uu % a.H);
+  const long sj = uu / a.H;
   const int s = (int)(sj / a.ntile), tile = (int)(sj % a.ntile);
   const int t0 = tile * 16;
-  const int rows = min(a.L - t0, 16);
+  const int rows = act ? min(a.L - t0, 16) : 0;
   const int len = min(max(a.length[s], 0), a.cap) - t0;             // held rows of this tile (may be <= 0)
-  const long row = (long)a.H * HD;
-  bf16_t* dst = (is_v ? a.v : a.k) + ((long)s * a.L + t0) * row + (long)h * HD + c * 8;
-  if (len <= 0) {
-    for (int i = 0; i < rows; ++i) *reinterpret_cast<uint4*>(dst + i * row) = make_uint4(0, 0, 0, 0);
-    return;
-  }
   const long head = (long)s * a.H + h;
   const float scale = (is_v ? a.vs : a.ks)[head * (a.cap >> a.bshift) + (t0 >> a.bshift)];
-  if (!is_v) {
-    const uint8_t* kp = a.k8 + (head * a.cap + t0) * HD + c * 8;
-    uint2 w[16];
+  char* mine = img[threadIdx.x >> 6];
+  const uint8_t* src = is_v ? a.v8 : a.k8;
+  const long base = (head * a.cap + t0) * HD;                       // K and V alike
+  uint4 w[8];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) w[i] = *reinterpret_cast<const uint2*>(kp + (long)i * HD);
+  for (int it = 0; it < 8; ++it) {                                  // consecutive lanes, consecutive pieces (a tile without rows: not looked at)
+    const int p16 = it * 64 + lane, u2 = p16 / HD, off = (p16 % HD) * 16;
+    const long b = __shfl(base, u2 * C, 64);
+    const int n = __shfl(len, u2 * C, 64);
+    if (n > 0) w[it] = *reinterpret_cast<const uint4*>(src + b + off);
+  }
+#pragma unroll
+  for (int it = 0; it < 8; ++it) {
+    const int p16 = it * 64 + lane;
+    *reinterpret_cast<uint4*>(mine + (p16 / HD) * US + (p16 % HD) * 16) = w[it];
+  }
+  __syncthreads();
+  const long row = (long)a.H * HD;
+  bf16_t* dst = (is_v ? a.v : a.k) + ((long)s * a.L + t0) * row + (long)h * HD + c * 8;
+  const char* at = mine + ui * US;
+  if (!is_v) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      if (i >= rows) break;
-      uint4 o = make_uint4(kv8_unpack2<DT, false>(w[i].x, scale), kv8_unpack2<DT, true>(w[i].x, scale), kv8_unpack2<DT, false>(w[i].y, scale),
-                           kv8_unpack2<DT, true>(w[i].y, scale));
+      const uint2 q = *reinterpret_cast<const uint2*>(at + i * HD + c * 8);
+      uint4 o = make_uint4(kv8_unpack2<DT, false>(q.x, scale), kv8_unpack2<DT, true>(q.x, scale), kv8_unpack2<DT, false>(q.y, scale),
+                           kv8_unpack2<DT, true>(q.y, scale));
       if (i >= len) o = make_uint4(0, 0, 0, 0);
-      *reinterpret_cast<uint4*>(dst + i * row) = o;
+      if (i < rows) *reinterpret_cast<uint4*>(dst + i * row) = o;
     }
     return;
   }
-  const uint8_t* vp = a.v8 + (head * (a.cap >> 4) + tile) * (HD * 16) + c * 128;
-  uint4 w[8];
 #pragma unroll
-  for (int ch = 0; ch < 8; ++ch) w[ch] = *reinterpret_cast<const uint4*>(vp + ch * 16);
+  for (int ch = 0; ch < 8; ++ch) w[ch] = *reinterpret_cast<const uint4*>(at + (c * 8 + ch) * 16);
 #pragma unroll
   for (int d = 0; d < 8; ++d) {                                     // positions 2 d, 2 d + 1
     uint32_t p[8];                                                  // per channel: the two positions as bf16
@@ -251,13 +279,11 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(ReadArgs a) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int i = 2 * d + e;
-      if (i < rows) {
-        const uint32_t sel = e ? 0x07060302u : 0x05040100u;
-        uint4 o = make_uint4(__builtin_amdgcn_perm(p[1], p[0], sel), __builtin_amdgcn_perm(p[3], p[2], sel), __builtin_amdgcn_perm(p[5], p[4], sel),
-                             __builtin_amdgcn_perm(p[7], p[6], sel));
-        if (i >= len) o = make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(dst + i * row) = o;
-      }
+      const uint32_t sel = e ? 0x07060302u : 0x05040100u;
+      uint4 o = make_uint4(__builtin_amdgcn_perm(p[1], p[0], sel), __builtin_amdgcn_perm(p[3], p[2], sel), __builtin_amdgcn_perm(p[5], p[4], sel),
+                           __builtin_amdgcn_perm(p[7], p[6], sel));
+      if (i >= len) o = make_uint4(0, 0, 0, 0);
+      if (i < rows) *reinterpret_cast<uint4*>(dst + i * row) = o;
     }
   }
 }
@@ -314,7 +340,8 @@ int neko_kv8_read_impl(const uint8_t* k8, const uint8_t* v8, const float* ks, co
   const int bshift = block == 16 ? 4 : block == 32 ? 5 : 6;
   ReadArgs a{k8, v8, ks, vs, k, v, length, S, H, cap, L, bshift, (L + 15) / 16, 0};
   a.units = (long)S * a.ntile * H;
-  const long blocks = (a.units * (hd / 8) + 255) / 256;
+  const long per_block = 4 * (64 / (hd / 8));
+  const long blocks = (a.units + per_block - 1) / per_block;
   if (blocks > 0x7fffffffL) return NEKO_ERR_UNSUPPORTED;
   const dim3 grid((unsigned)blocks, 2);
 #define NEKO_KV8_READ(HD)                                                                              \

@@ -7,6 +7,7 @@ immediately.  Shape/dtype preconditions are asserted before the call (SURVEY.md 
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 from typing import Optional
 
@@ -606,20 +607,43 @@ def patch_pos_add_bwd(dout, hpos, wpos, d_row, d_col, sorted_rows=None):
 
 
 # ---- serving: 8-bit key / value cache, attention over it, verification of drafted tokens ---------------------------------------------
+# A decode step is a few microseconds of kernel per call, so these wrappers keep their own cost down: one combined test per argument (the
+# detailed message is worked out only when it fails), memoised workspace sizes (functions of the sizes alone), entry points bound once.
 _KV8_DTYPES = {torch.float8_e4m3fn: 0, torch.int8: 1}
+_I32, _I64, _F32 = torch.int32, torch.int64, torch.float32
 
 
-def _here(t: torch.Tensor, name: str) -> None:
+def _here(t: torch.Tensor, name: str) -> int:
     """The launch goes to the current device's current stream: the tensor has to live there."""
     assert t.is_cuda, f"{name} must be a device tensor"
-    assert t.device.index == torch._C._cuda_getDevice(), f"{name} is on {t.device}, the current device is cuda:{torch._C._cuda_getDevice()}"
+    dev = torch._C._cuda_getDevice()
+    assert t.get_device() == dev, f"{name} is on {t.device}, the current device is cuda:{dev}"
+    return dev
 
 
-def _ints(t: Optional[torch.Tensor], n: int, name: str, dtype=torch.int32) -> None:
-    if t is not None:
+def _vec(t: Optional[torch.Tensor], n: int, name: str, dev: int, dtype=torch.int32):
+    """Address of `n` contiguous values of `dtype` on device `dev` (None stays None)."""
+    if t is None:
+        return None
+    if not (t.dtype is dtype and t.numel() == n and t.get_device() == dev and t.is_contiguous()):
         _here(t, name)
         assert t.dtype == dtype, f"{name} must be {dtype}, got {t.dtype}"
-        assert t.numel() == n and t.is_contiguous(), f"{name} must hold {n} contiguous values"
+        raise AssertionError(f"{name} must hold {n} contiguous values, got {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _raw(dev: int) -> int:
+    return _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
+
+
+@functools.lru_cache(maxsize=None)
+def _entry(name: str):
+    return getattr(_lib.load(), name)
+
+
+@functools.lru_cache(maxsize=4096)
+def _size(name: str, *sizes: int) -> int:
+    return int(_entry(name)(*sizes))
 
 
 class KV8Cache:
@@ -630,76 +654,83 @@ class KV8Cache:
     per block of 16 / 32 / 64 positions and head.  The cache does not know how much of it is filled: positions are arguments of kv8_append,
     kv8_read and attn_kv8 (device tensors, so that a captured step can advance them)."""
 
+    __slots__ = ("k", "v", "k_scale", "v_scale", "nseq", "heads", "cap", "hd", "block", "dtype", "device", "_args")
+
     def __init__(self, nseq: int, heads: int, cap: int, hd: int, dtype=torch.float8_e4m3fn, block: int = 32, device="cuda"):
         assert dtype in _KV8_DTYPES, f"cache dtype must be one of {list(_KV8_DTYPES)}, got {dtype}"
         assert nseq > 0 and heads > 0 and cap > 0 and cap % 64 == 0, "cap must be a positive multiple of 64"
         assert hd in (32, 64, 128) and block in (16, 32, 64), "hd must be 32 / 64 / 128, block 16 / 32 / 64"
         u8 = torch.zeros((2, nseq, heads, cap, hd), dtype=torch.uint8, device=device)
         sc = torch.ones((2, nseq, heads, cap // block), dtype=torch.float32, device=device)
-        self._set(u8[0].view(dtype), u8[1].view(nseq, heads, cap // 16, hd, 16).view(dtype), sc[0], sc[1])
+        self._set(u8[0].view(dtype), u8[1].view(nseq, heads, cap // 16, hd, 16).view(dtype), sc[0], sc[1], nseq, heads, cap, hd, block)
 
-    def _set(self, k, v, k_scale, v_scale):
+    def _set(self, k, v, k_scale, v_scale, S, H, cap, hd, block):
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.nseq, self.heads, self.cap, self.hd = k.shape
-        self.block = self.cap // k_scale.shape[2]
+        self.nseq, self.heads, self.cap, self.hd, self.block = S, H, cap, hd, block
         self.dtype, self.device = k.dtype, k.device
         # the leading arguments of every entry point of the cache
-        self._args = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), _KV8_DTYPES[k.dtype], self.nseq, self.heads, self.cap,
-                      self.hd, self.block)
+        self._args = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), _KV8_DTYPES[k.dtype], S, H, cap, hd, block)
 
     @classmethod
     def from_tensors(cls, k, v, k_scale, v_scale) -> "KV8Cache":
         """A cache over tensors that the caller holds (no copy): k, v, k_scale, v_scale as in the class description, contiguous."""
-        assert k.dim() == 4 and k_scale.dim() == 3 and k.dtype in _KV8_DTYPES and v.dtype == k.dtype, "k [nseq, heads, cap, hd] in e4m3 or int8"
+        dt, dev = k.dtype, k.device
+        assert dt in _KV8_DTYPES and v.dtype is dt and k.dim() == 4 and k_scale.dim() == 3, "k [nseq, heads, cap, hd] and v in e4m3 or int8"
         S, H, cap, hd = k.shape
         nb = k_scale.shape[2]
         assert cap > 0 and cap % 64 == 0 and hd in (32, 64, 128), "cap must be a positive multiple of 64, hd 32 / 64 / 128"
         assert nb > 0 and cap % nb == 0 and cap // nb in (16, 32, 64), "one scale per 16 / 32 / 64 positions"
-        assert tuple(v.shape) == (S, H, cap // 16, hd, 16), f"v must be {(S, H, cap // 16, hd, 16)}, got {tuple(v.shape)}"
-        assert tuple(k_scale.shape) == (S, H, nb) and tuple(v_scale.shape) == (S, H, nb), "scales must be [nseq, heads, cap / block]"
-        assert k_scale.dtype == torch.float32 and v_scale.dtype == torch.float32, "scales must be float32"
+        assert v.shape == (S, H, cap // 16, hd, 16), f"v must be {(S, H, cap // 16, hd, 16)}, got {tuple(v.shape)}"
+        assert k_scale.shape == v_scale.shape == (S, H, nb), "scales must be [nseq, heads, cap / block]"
+        assert k_scale.dtype is _F32 and v_scale.dtype is _F32, "scales must be float32"
         assert k.is_contiguous() and v.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous(), "cache tensors must be contiguous"
-        assert k.device == v.device == k_scale.device == v_scale.device, "cache tensors must be on one device"
+        assert v.device == dev and k_scale.device == dev and v_scale.device == dev, "cache tensors must be on one device"
         assert (k.data_ptr() | v.data_ptr()) % 16 == 0, "cache tensors must be 16-byte aligned"
         c = cls.__new__(cls)
-        c._set(k, v, k_scale, v_scale)
+        c._set(k, v, k_scale, v_scale, S, H, cap, hd, cap // nb)
         return c
 
-    def row_strides(self, x: torch.Tensor, heads: int, name: str):
-        """(rows per sequence, sequence stride, row stride) of x [nseq, T, heads, hd] bf16 whose heads lie side by side (a view of a fused
-        projection will do)."""
-        _here(x, name)
-        assert x.dtype == BF16, f"{name} must be {BF16}, got {x.dtype}"
-        assert x.dim() == 4 and x.shape[0] == self.nseq and x.shape[2] == heads and x.shape[3] == self.hd and x.shape[1] > 0, \
-            f"{name} must be [{self.nseq}, T, {heads}, {self.hd}], got {tuple(x.shape)}"
+    def row_strides(self, x: torch.Tensor, heads: int, name: str, dev: int):
+        """(rows per sequence, sequence stride, row stride, address) of x [nseq, T, heads, hd] bf16 whose heads lie side by side (a view of a
+        fused projection will do)."""
+        if x.get_device() != dev or x.dtype is not BF16 or x.dim() != 4:
+            _here(x, name)
+            assert x.dtype == BF16, f"{name} must be {BF16}, got {x.dtype}"
+        S, T, H, hd = x.shape if x.dim() == 4 else (-1, 0, 0, 0)
+        assert S == self.nseq and H == heads and hd == self.hd and T > 0, f"{name} must be [{self.nseq}, T, {heads}, {self.hd}], got {tuple(x.shape)}"
         ss, st, sh, sc = x.stride()
-        assert sc == 1 and (sh == self.hd or heads == 1), f"{name}: the heads of a row must be contiguous"
-        T = x.shape[1]
-        st = st if T > 1 else heads * self.hd
-        ss = ss if self.nseq > 1 else T * st
-        assert st % 8 == 0 and ss % 8 == 0 and x.data_ptr() % 16 == 0, f"{name}: rows must be 16-byte aligned"
-        return T, ss, st
+        assert sc == 1 and (sh == hd or H == 1), f"{name}: the heads of a row must be contiguous"
+        if T == 1:
+            st = H * hd
+        if S == 1:
+            ss = T * st
+        p = x.data_ptr()
+        assert (st | ss) % 8 == 0 and p % 16 == 0, f"{name}: rows must be 16-byte aligned"
+        return T, ss, st, p
 
 
 def kv8_append(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, n_new: Optional[torch.Tensor] = None) -> None:
     """Quantise rows 0 .. n_new[s]-1 of k, v [nseq, T, heads, hd] (bf16) into positions pos[s] .. of every sequence; see neko_kv8_append."""
-    T, k_ss, k_st = cache.row_strides(k, cache.heads, "k")
-    Tv, v_ss, v_st = cache.row_strides(v, cache.heads, "v")
+    dev = _here(cache.k, "cache")
+    S = cache.nseq
+    T, k_ss, k_st, kp = cache.row_strides(k, cache.heads, "k", dev)
+    Tv, v_ss, v_st, vp = cache.row_strides(v, cache.heads, "v", dev)
     assert T == Tv, "k and v must have the same number of rows"
-    _here(cache.k, "cache")
-    _ints(pos, cache.nseq, "pos")
-    _ints(n_new, cache.nseq, "n_new")
-    _lib.call("neko_kv8_append", *cache._args, k.data_ptr(), k_ss, k_st, v.data_ptr(), v_ss, v_st, pos.data_ptr(), _p(n_new), T, _stream())
+    rc = _entry("neko_kv8_append")(*cache._args, kp, k_ss, k_st, vp, v_ss, v_st, _vec(pos, S, "pos", dev), _vec(n_new, S, "n_new", dev), T, _raw(dev))
+    if rc:
+        _lib.check(rc, "neko_kv8_append")
 
 
 def kv8_read(cache: KV8Cache, length: torch.Tensor, L: int):
     """Rows 0 .. L-1 of every sequence as bf16 -> (k, v) [nseq, L, heads, hd]; rows at and behind length[s] are 0; see neko_kv8_read."""
     assert 0 < L <= cache.cap, f"L must be in 1 .. {cache.cap}"
-    _here(cache.k, "cache")
-    _ints(length, cache.nseq, "length")
+    dev = _here(cache.k, "cache")
+    n = _vec(length, cache.nseq, "length", dev)
     k = torch.empty((cache.nseq, L, cache.heads, cache.hd), dtype=BF16, device=cache.device)
     v = torch.empty_like(k)
-    _lib.call("neko_kv8_read", *cache._args, length.data_ptr(), int(L), k.data_ptr(), v.data_ptr(), _stream())
+    rc = _entry("neko_kv8_read")(*cache._args, n, L, k.data_ptr(), v.data_ptr(), _raw(dev))
+    if rc:
+        _lib.check(rc, "neko_kv8_read")
     return k, v
 
 
@@ -709,34 +740,37 @@ def attn_kv8(cache: KV8Cache, q: torch.Tensor, pos: torch.Tensor, n_new: Optiona
     first); causal, keys from start[s] on, optionally a sliding `window` with the first `sinks` keys kept visible.  Rows at and behind
     n_new[s] of `out` are left as they are (a fresh output holds zeros there).  max_len: host-known bound on pos + T, sizes the launch.  See
     neko_attn_kv8."""
-    assert q.dim() == 4 and q.shape[2] % cache.heads == 0 and q.shape[2] > 0, f"q must be [{cache.nseq}, T, G * {cache.heads}, {cache.hd}]"
-    HG = q.shape[2]
-    T, q_ss, q_st = cache.row_strides(q, HG, "q")
-    assert T <= cache.cap, "more rows than the cache has positions"
+    dev = _here(cache.k, "cache")
+    S, H, cap, hd = cache.nseq, cache.heads, cache.cap, cache.hd
+    HG = q.shape[2] if q.dim() == 4 else 0
+    assert HG > 0 and HG % H == 0, f"q must be [{S}, T, G * {H}, {hd}], got {tuple(q.shape)}"
+    T, q_ss, q_st, qp = cache.row_strides(q, HG, "q", dev)
+    assert T <= cap, "more rows than the cache has positions"
     assert window >= 0 and sinks >= 0 and (sinks == 0 or window > 0), "sinks need a window"
     assert scale is None or scale > 0.0, "scale must be positive"
-    _here(cache.k, "cache")
-    _ints(pos, cache.nseq, "pos")
-    _ints(n_new, cache.nseq, "n_new")
-    _ints(start, cache.nseq, "start")
     if out is None:
-        out = (torch.empty if n_new is None else torch.zeros)((cache.nseq, T, HG, cache.hd), dtype=BF16, device=cache.device)
-    To, o_ss, o_st = cache.row_strides(out, HG, "out")
+        out = (torch.empty if n_new is None and start is None else torch.zeros)((S, T, HG, hd), dtype=BF16, device=cache.device)
+    To, o_ss, o_st, op = cache.row_strides(out, HG, "out", dev)
     assert To == T, "out must have q's rows"
-    lib = _lib.load()
-    G = HG // cache.heads
-    nws = lib.neko_attn_kv8_ws_floats(cache.nseq, cache.heads, G, cache.cap, cache.hd, T, int(window), int(sinks), int(max_len))
-    ws = torch.empty(nws, dtype=torch.float32, device=cache.device) if nws else None
-    _lib.call("neko_attn_kv8", *cache._args, q.data_ptr(), q_ss, q_st, out.data_ptr(), o_ss, o_st, G, T, pos.data_ptr(), _p(n_new), _p(start),
-              int(window), int(sinks), float(scale) if scale is not None else cache.hd ** -0.5, int(max_len), _p(ws), nws, _stream())
+    G = HG // H
+    nws = _size("neko_attn_kv8_ws_floats", S, H, G, cap, hd, T, window, sinks, max_len)
+    ws = torch.empty(nws, dtype=_F32, device=cache.device) if nws else None
+    rc = _entry("neko_attn_kv8")(*cache._args, qp, q_ss, q_st, op, o_ss, o_st, G, T, _vec(pos, S, "pos", dev), _vec(n_new, S, "n_new", dev),
+                                 _vec(start, S, "start", dev), window, sinks, scale if scale is not None else hd ** -0.5, max_len,
+                                 ws.data_ptr() if nws else None, nws, _raw(dev))
+    if rc:
+        _lib.check(rc, "neko_attn_kv8")
     return out
 
 
-def _logit_rows(x: torch.Tensor, shape, name: str):
-    _here(x, name)
-    assert x.dtype in (torch.float32, BF16), f"{name} must be float32 or bfloat16, got {x.dtype}"
-    assert x.dim() == 3 and tuple(x.shape) == shape, f"{name} must be {list(shape)}, got {list(x.shape)}"
-    assert x.stride(2) == 1 or x.shape[2] == 1, f"{name}: a row's logits must be contiguous"
+def _logit_rows(x: torch.Tensor, shape, name: str, dev: int):
+    if x.get_device() != dev or x.dim() != 3:
+        _here(x, name)
+    assert x.dtype is _F32 or x.dtype is BF16, f"{name} must be float32 or bfloat16, got {x.dtype}"
+    assert x.shape == shape, f"{name} must be {list(shape)}, got {list(x.shape)}"
+    sb, sr, sc = x.stride()
+    assert sc == 1 or shape[2] == 1, f"{name}: a row's logits must be contiguous"
+    return x.data_ptr(), sb, sr
 
 
 def verify_draft(logits: torch.Tensor, tokens: torch.Tensor, draft_logits: Optional[torch.Tensor] = None, u: Optional[torch.Tensor] = None,
@@ -750,27 +784,26 @@ def verify_draft(logits: torch.Tensor, tokens: torch.Tensor, draft_logits: Optio
     assert B > 0 and 0 < K <= 62, "1 to 62 drafted tokens"
     V = logits.shape[-1]
     assert V > 0 and temperature >= 0.0, "temperature must not be negative"
-    _logit_rows(logits, (B, K + 1, V), "logits")
-    _ints(tokens, B * K, "tokens", torch.int64)
-    _ints(n_draft, B, "n_draft")
+    dev = _here(logits, "logits")
+    tp, t_sb, t_sr = _logit_rows(logits, (B, K + 1, V), "logits", dev)
+    dp, d_sb, d_sr = None, 0, 0
     if temperature > 0:
         assert u is not None and r is not None, "sampling needs u [B, K] and r [B]"
-        _ints(u, B * K, "u", torch.float32)
-        _ints(r, B, "r", torch.float32)
         if draft_logits is not None:
-            _logit_rows(draft_logits, (B, K, V), "draft_logits")
-            assert draft_logits.dtype == logits.dtype, "logits and draft_logits must have one type"
+            dp, d_sb, d_sr = _logit_rows(draft_logits, (B, K, V), "draft_logits", dev)
+            assert draft_logits.dtype is logits.dtype, "logits and draft_logits must have one type"
     else:
-        draft_logits = None
-    accepted = torch.empty(B, dtype=torch.int32, device=logits.device)
-    out = torch.empty((B, K + 1), dtype=torch.int64, device=logits.device)
-    lib = _lib.load()
-    nws = lib.neko_verify_draft_ws_bytes(B, K, V)
-    ws = torch.empty(nws, dtype=torch.uint8, device=logits.device)
-    d = draft_logits
-    _lib.call("neko_verify_draft", logits.data_ptr(), logits.stride(0), logits.stride(1), _p(d), d.stride(0) if d is not None else 0,
-              d.stride(1) if d is not None else 0, int(logits.dtype == BF16), B, K, V, tokens.data_ptr(), _p(u), _p(r), _p(n_draft),
-              float(temperature), accepted.data_ptr(), out.data_ptr(), ws.data_ptr(), nws, _stream())
+        u = r = None
+    where = logits.device
+    accepted = torch.empty(B, dtype=_I32, device=where)
+    out = torch.empty((B, K + 1), dtype=_I64, device=where)
+    nws = _size("neko_verify_draft_ws_bytes", B, K, V)
+    ws = torch.empty(nws, dtype=torch.uint8, device=where)
+    rc = _entry("neko_verify_draft")(tp, t_sb, t_sr, dp, d_sb, d_sr, logits.dtype is BF16, B, K, V, _vec(tokens, B * K, "tokens", dev, _I64),
+                                     _vec(u, B * K, "u", dev, _F32), _vec(r, B, "r", dev, _F32), _vec(n_draft, B, "n_draft", dev), temperature,
+                                     accepted.data_ptr(), out.data_ptr(), ws.data_ptr(), nws, _raw(dev))
+    if rc:
+        _lib.check(rc, "neko_verify_draft")
     return accepted, out
 
 
@@ -780,28 +813,27 @@ def distill_topk(z: torch.Tensor, V: int, Vpad: int, t_val: Optional[torch.Tenso
                  dlogits: Optional[torch.Tensor] = None) -> None:
     """Rows of student logits z [R, >= Vpad] (bf16 or fp32, columns < V valid) against a teacher's top logits t_val [R, k] fp32 at t_idx [R, k]
     int32: loss_row [R] fp32 = (1 - hard) tau^2 KL + hard CE(target), dlogits (z's type, may be z) = weight * gradient; see neko_distill_topk."""
-    _here(z, "z")
-    assert z.dtype in (torch.float32, BF16), f"z must be float32 or bfloat16, got {z.dtype}"
-    assert z.dim() == 2 and z.stride(1) == 1 and z.shape[1] >= Vpad >= V > 0, "z must be [R, >= Vpad] with contiguous rows"
+    dev = _here(z, "z")
+    assert z.dtype is _F32 or z.dtype is BF16, f"z must be float32 or bfloat16, got {z.dtype}"
+    assert z.dim() == 2 and z.shape[1] >= Vpad >= V > 0 and z.stride(1) == 1, "z must be [R, >= Vpad] with contiguous rows"
     R = z.shape[0]
     assert R > 0 and tau > 0.0 and 0.0 <= hard <= 1.0, "tau must be positive, hard in [0, 1]"
     assert loss_row is not None or dlogits is not None, "nothing to compute"
-    k = 0
+    k, tv, ti = 0, None, None
     if hard < 1.0:
         assert t_val is not None and t_idx is not None and t_val.dim() == 2 and t_val.shape == t_idx.shape, "t_val and t_idx must be [R, k]"
         k = t_val.shape[1]
         assert 0 < k <= 1024, "1 to 1024 teacher entries"
-        _ints(t_val, R * k, "t_val", torch.float32)
-        _ints(t_idx, R * k, "t_idx")
-    if hard > 0.0:
-        assert target is not None, "hard > 0 needs target"
-    _ints(target, R, "target", torch.int64)
-    _ints(weight, R, "weight", torch.float32)
-    _ints(loss_row, R, "loss_row", torch.float32)
+        tv, ti = _vec(t_val, R * k, "t_val", dev, _F32), _vec(t_idx, R * k, "t_idx", dev)
+    assert hard == 0.0 or target is not None, "hard > 0 needs target"
+    ldz, ldd, dp = (z.stride(0) if R > 1 else z.shape[1]), 0, None
     if dlogits is not None:
-        _here(dlogits, "dlogits")
-        assert dlogits.dtype == z.dtype and dlogits.dim() == 2 and dlogits.shape[0] == R and dlogits.shape[1] >= Vpad and dlogits.stride(1) == 1, \
+        if dlogits.get_device() != dev or dlogits.dtype is not z.dtype:
+            _here(dlogits, "dlogits")
+        assert dlogits.dtype is z.dtype and dlogits.dim() == 2 and dlogits.shape[0] == R and dlogits.shape[1] >= Vpad and dlogits.stride(1) == 1, \
             "dlogits must be like z"
-    _lib.call("neko_distill_topk", z.data_ptr(), max(z.stride(0), Vpad) if R == 1 else z.stride(0), int(z.dtype == BF16), R, V, Vpad, _p(t_val) if k else None,
-              _p(t_idx) if k else None, k, weight.data_ptr(), float(tau), _p(target), float(hard), _p(loss_row), _p(dlogits),
-              0 if dlogits is None else (max(dlogits.stride(0), Vpad) if R == 1 else dlogits.stride(0)), _stream())
+        ldd, dp = (dlogits.stride(0) if R > 1 else dlogits.shape[1]), dlogits.data_ptr()
+    rc = _entry("neko_distill_topk")(z.data_ptr(), ldz, z.dtype is BF16, R, V, Vpad, tv, ti, k, _vec(weight, R, "weight", dev, _F32), tau,
+                                     _vec(target, R, "target", dev, _I64), hard, _vec(loss_row, R, "loss_row", dev, _F32), dp, ldd, _raw(dev))
+    if rc:
+        _lib.check(rc, "neko_distill_topk")
