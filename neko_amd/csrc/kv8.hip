@@ -51,6 +51,15 @@ __device__ __forceinline__ uint32_t pkmax_u16(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
 }
 
+// bf16 bits of the largest magnitude -> the scale: am = (1 + m / 128) 2^(x - 127); qmax = 1.75 * 2^8 | (1 + 126 / 128) * 2^6
+template <int DT>
+__device__ __forceinline__ float scale_of(uint32_t am) {
+  const int x = (int)(am >> 7), m = (int)(am & 0x7f);
+  int e = DT == 0 ? x - 127 - 8 + (m > 96) : x - 127 - 6 + (m > 126);
+  if (x == 0 || e < -100) e = -100;
+  return __uint_as_float((uint32_t)(e + 127) << 23);
+}
+
 // a unit (one block of one head, K or V) on its way out: where it goes, its first position, the new positions [pc, end) (end < 0: nothing),
 // and the factor of its older codes if their grid grew (0: it did not)
 struct UnitOut { long base; int b0, pc, end; float ratio; };
@@ -113,11 +122,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
   for (int o = 1; o < C; o <<= 1) am = max(am, (uint32_t)__shfl_xor((int)am, o, 64));
 #pragma unroll
   for (int o = C * U; o < 64; o <<= 1) am = max(am, (uint32_t)__shfl_xor((int)am, o, 64));
-  // bf16 bits -> exponent of the scale: am = (1 + m / 128) 2^(x - 127); qmax = 1.75 * 2^8 | (1 + 126 / 128) * 2^6
-  const int x = (int)(am >> 7), m = (int)(am & 0x7f);
-  int e = DT == 0 ? x - 127 - 8 + (m > 96) : x - 127 - 6 + (m > 126);
-  if (x == 0 || e < -100) e = -100;
-  float scale = __uint_as_float((uint32_t)(e + 127) << 23);
+  float scale = scale_of<DT>(am);
   const long head = (long)s * a.H + h;
   float* sp = (is_v ? a.vs : a.ks) + head * (a.cap >> a.bshift) + blk;
   const bool held = act && b0 < pc;                                 // the block holds older rows
@@ -204,6 +209,70 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
       }
     }
     *dst = make_uint4(q[0], q[1], q[2], q[3]);
+  }
+}
+
+// One row a sequence (a decode step): latency is all there is, and the general kernel's image, exchange and read-change-write of a tile cost four
+// round trips to memory where this one has two (positions; row and scale).  A lane owns 8 channels of one head's key or value; V's bytes are
+// stored one by one.
+template <int HD, int DT>
+__global__ __launch_bounds__(256) void kv8_append_row_kernel(AppendArgs a) {
+  constexpr int C = HD / 8;
+  const bool is_v = blockIdx.y != 0;
+  const long id = (long)blockIdx.x * 256 + threadIdx.x;
+  const int c = (int)(id % C);
+  const long u = id / C;
+  const long uu = min(u, a.units - 1);
+  const int h = (int)(uu % a.H), s = (int)(uu / a.H);
+  const int p = a.pos[s];
+  const bool act = u < a.units && p >= 0 && p < a.cap && (!a.n_new || a.n_new[s] > 0);
+  const int pc = min(max(p, 0), a.cap - 1);
+  uint4 raw = *reinterpret_cast<const uint4*>((is_v ? a.v : a.k) + (is_v ? a.v_ss : a.k_ss) * s + (long)h * HD + c * 8);
+  const long head = (long)s * a.H + h;
+  const int blk = pc >> a.bshift, b0 = blk << a.bshift;
+  float* sp = (is_v ? a.vs : a.ks) + head * (a.cap >> a.bshift) + blk;
+  const float there = *sp;
+  raw.x = tame2(raw.x); raw.y = tame2(raw.y); raw.z = tame2(raw.z); raw.w = tame2(raw.w);
+  const uint32_t mx = pkmax_u16(pkmax_u16(raw.x & 0x7fff7fffu, raw.y & 0x7fff7fffu), pkmax_u16(raw.z & 0x7fff7fffu, raw.w & 0x7fff7fffu));
+  uint32_t am = max(mx & 0xffffu, mx >> 16);
+#pragma unroll
+  for (int o = 1; o < C; o <<= 1) am = max(am, (uint32_t)__shfl_xor((int)am, o, 64));
+  if (!act) return;
+  float scale = scale_of<DT>(am);
+  const bool held = b0 < pc;
+  if (held) scale = fmaxf(scale, there);
+  const float inv = 1.0f / scale;
+  if (c == 0) *sp = scale;                 // (the head's lanes are in one wave and have read it)
+  uint8_t* kp = a.k8 + (head * a.cap) * HD + c * 8;
+  uint8_t* vp = a.v8 + (head * a.cap) * HD + c * 128;
+  if (held && scale > there) {             // the grid grew: the block's older codes once more
+    const float ratio = there * inv;
+    auto again = [&](uint32_t w) {
+      return kv8_pack4<DT>(kv8_code<DT>(w & 0xff) * ratio, kv8_code<DT>((w >> 8) & 0xff) * ratio, kv8_code<DT>((w >> 16) & 0xff) * ratio,
+                           kv8_code<DT>(w >> 24) * ratio);
+    };
+    if (!is_v) {
+      for (int t = b0; t < pc; ++t) {
+        uint2* q = reinterpret_cast<uint2*>(kp + (long)t * HD);
+        *q = make_uint2(again(q->x), again(q->y));
+      }
+    } else {
+      for (int t = b0; t < pc; t += 4)
+        for (int ch = 0; ch < 8; ++ch) {
+          uint32_t* q = reinterpret_cast<uint32_t*>(vp + (long)(t >> 4) * (HD * 16) + ch * 16 + (t & 15));
+          const uint32_t old = pc - t >= 4 ? 0xffffffffu : (1u << (8 * (pc - t))) - 1u;
+          *q = (again(*q) & old) | (*q & ~old);
+        }
+    }
+  }
+  const uint2 w = make_uint2(kv8_pack4<DT>(lo_f(raw.x) * inv, hi_f(raw.x) * inv, lo_f(raw.y) * inv, hi_f(raw.y) * inv),
+                             kv8_pack4<DT>(lo_f(raw.z) * inv, hi_f(raw.z) * inv, lo_f(raw.w) * inv, hi_f(raw.w) * inv));
+  if (!is_v) {
+    *reinterpret_cast<uint2*>(kp + (long)pc * HD) = w;
+  } else {
+    uint8_t* q = vp + (long)(pc >> 4) * (HD * 16) + (pc & 15);
+#pragma unroll
+    for (int ch = 0; ch < 8; ++ch) q[ch * 16] = (uint8_t)((ch < 4 ? w.x : w.y) >> (8 * (ch & 3)));
   }
 }
 
@@ -320,6 +389,18 @@ int neko_kv8_append_impl(uint8_t* k8, uint8_t* v8, float* ks, float* vs, int dty
   T = min(T, cap);
   AppendArgs a{k8, v8, ks, vs, k, v, k_ss, k_st, v_ss, v_st, pos, n_new, S, H, cap, T, bshift, (T - 1 + block - 1) / block + 1, 0};
   a.units = (long)S * a.nslots * H;
+  if (T == 1) {
+    const dim3 grid((unsigned)((a.units * (hd / 8) + 255) / 256), 2);
+#define NEKO_KV8_ROW(HD)                                                                                    \
+  if (dtype == 0) hipLaunchKernelGGL((kv8_append_row_kernel<HD, 0>), grid, dim3(256), 0, s, a);             \
+  else hipLaunchKernelGGL((kv8_append_row_kernel<HD, 1>), grid, dim3(256), 0, s, a)
+    if (hd == 32) { NEKO_KV8_ROW(32); }
+    else if (hd == 64) { NEKO_KV8_ROW(64); }
+    else { NEKO_KV8_ROW(128); }
+#undef NEKO_KV8_ROW
+    NEKO_CHECK_LAUNCH();
+    return NEKO_OK;
+  }
   const int per_wave = 64 / ((hd / 8) * (block / 16));
   const long blocks = (a.units + 4 * per_wave - 1) / (4 * per_wave);
   if (blocks > 0x7fffffffL) return NEKO_ERR_UNSUPPORTED;
