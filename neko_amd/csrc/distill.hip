@@ -103,8 +103,8 @@ __global__ __launch_bounds__(NT, NCH <= 7 ? 8 : 4) void distill_kernel(DistillAr
   constexpr int N = P::N, NW = NT / 64;
   constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
   __shared__ float red[3][NW];
-  __shared__ float s_t[KMAX];
-  __shared__ int s_i[KMAX];
+  __shared__ int2 s_e[KMAX];                           // teacher entries: index (-1: none), probability
+  __shared__ float s_z[KMAX];                          // the student's logit there
   __shared__ float s_teacher[2];                       // sum t log t; 1 if there is a teacher
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const T* z = (const T*)a.z + (long)row * a.ldz;
@@ -146,6 +146,15 @@ __global__ __launch_bounds__(NT, NCH <= 7 ? 8 : 4) void distill_kernel(DistillAr
     }
   };
   const int rounds = NCH > 0 ? NCH : (nch + NT - 1) / NT;
+  // the student's logits at the teacher's entries and at the label, read before anything is overwritten
+  const float zy = has_y ? P::one(z + y) : 0.f;
+  if (soft_w != 0.f) {
+#pragma unroll 1
+    for (int j = tid; j < a.k; j += NT) {
+      const int ix = a.t_idx[(long)row * a.k + j];
+      s_z[j] = P::one(z + (ix >= 0 && ix < a.V ? ix : 0));
+    }
+  }
 
   // the teacher's entries (wave 0): index, probability
   if (soft_w != 0.f) {
@@ -156,8 +165,7 @@ __global__ __launch_bounds__(NT, NCH <= 7 ? 8 : 4) void distill_kernel(DistillAr
       for (int j = lane; j < a.k; j += 64) {
         const int ix = a.t_idx[(long)row * a.k + j];
         const float v = ix >= 0 && ix < a.V ? a.t_val[(long)row * a.k + j] : -INFINITY;
-        s_i[j] = v == -INFINITY ? -1 : ix;
-        s_t[j] = v;
+        s_e[j] = make_int2(v == -INFINITY ? -1 : ix, __float_as_int(v));
         tm = fmaxf(tm, v);
       }
       tm = wave_max(tm);
@@ -165,19 +173,19 @@ __global__ __launch_bounds__(NT, NCH <= 7 ? 8 : 4) void distill_kernel(DistillAr
       float ts = 0.f;
 #pragma unroll 1
       for (int j = lane; j < a.k; j += 64)
-        if (s_i[j] >= 0) ts += __expf((s_t[j] - tm) * it);
+        if (s_e[j].x >= 0) ts += __expf((__int_as_float(s_e[j].y) - tm) * it);
       ts = wave_sum(ts);
       const float inv = any ? 1.0f / ts : 0.f, lts = logf(ts);
       float acc = 0.f;
 #pragma unroll 1
       for (int j = lane; j < a.k; j += 64) {
         float t = 0.f;
-        if (s_i[j] >= 0) {
-          const float lt = (s_t[j] - tm) * it;
+        if (s_e[j].x >= 0) {
+          const float lt = (__int_as_float(s_e[j].y) - tm) * it;
           t = __expf(lt) * inv;
           if (t > 0.f) acc += t * (lt - lts);          // sum t log t
         }
-        s_t[j] = t;
+        s_e[j].y = __float_as_int(t);
       }
       acc = wave_sum(acc);
       if (lane == 0) { s_teacher[0] = acc; s_teacher[1] = any ? 1.f : 0.f; }
@@ -250,41 +258,19 @@ __global__ __launch_bounds__(NT, NCH <= 7 ? 8 : 4) void distill_kernel(DistillAr
     float acc = 0.f;
     if (soft)
 #pragma unroll 1
-      for (int j = lane; j < a.k; j += 64)
-        if (s_t[j] > 0.f) acc += s_t[j] * fmaf(P::one(z + s_i[j]), c1, b1);
+      for (int j = lane; j < a.k; j += 64) {
+        const float t = __int_as_float(s_e[j].y);
+        if (t > 0.f) acc += t * fmaf(s_z[j], c1, b1);
+      }
     acc = wave_sum(acc);
     if (lane == 0) {
       float loss = 0.f;
       if (soft) loss += soft_w * a.tau * a.tau * (s_teacher[0] + LN2 * (log2f(sum_soft) - acc));
-      if (has_y) loss += a.hard * LN2 * (log2f(sum_hard) - (TWO ? fmaf(P::one(z + y), LOG2E, b2) : fmaf(P::one(z + y), c1, b1)));
+      if (has_y) loss += a.hard * LN2 * (log2f(sum_hard) - (TWO ? fmaf(zy, LOG2E, b2) : fmaf(zy, c1, b1)));
       a.loss_row[row] = loss;
     }
   }
   if (!dz) return;
-  // this thread's sparse results (their logits are read before the dense pass overwrites them in place)
-  constexpr int MAXJ = (KMAX + NT) / NT;               // k + 1 entries over NT threads
-  float fix[MAXJ];
-  int at[MAXJ];
-#pragma unroll
-  for (int q = 0; q < MAXJ; ++q) {
-    const int j = tid + q * NT;
-    at[q] = -1;
-    fix[q] = 0.f;
-    if (j < a.k && soft) at[q] = s_i[j];
-    if (j == a.k && has_y) at[q] = (int)y;
-    if (at[q] >= 0) {
-      const float x = P::one(z + at[q]);
-      float t = 0.f;
-      if (soft)
-#pragma unroll 4
-        for (int i = 0; i < a.k; ++i) t += s_i[i] == at[q] ? s_t[i] : 0.f;
-      float g = 0.f;
-      if (soft) g += w * (fs * __builtin_amdgcn_exp2f(fmaf(x, c1, b1)) - soft_w * a.tau * t);
-      if (has_y) g += w * (fh * __builtin_amdgcn_exp2f(TWO ? fmaf(x, LOG2E, b2) : fmaf(x, c1, b1)) - (at[q] == (int)y ? a.hard : 0.f));
-      fix[q] = g;
-    }
-  }
-  __syncthreads();                                      // every sparse logit is read
   keep_packed();
   // bf16 results: the factor of a term goes into its exponent, the sign of the weight into the packing.  fp32 results multiply (an exponent of 40
   // is held to 2^-19 only)
@@ -318,10 +304,28 @@ __global__ __launch_bounds__(NT, NCH <= 7 ? 8 : 4) void distill_kernel(DistillAr
       __builtin_nontemporal_store((u32x4_v){o.x, o.y, o.z, o.w}, reinterpret_cast<u32x4_v*>(dz) + c);
     }
   }
-  __syncthreads();                                      // the dense values are written
-#pragma unroll
-  for (int q = 0; q < MAXJ; ++q)
-    if (at[q] >= 0) dz[at[q]] = P::store(fix[q]);
+  // the sparse results replace the dense ones: the dense terms once more, minus everything the teacher and the label have at this place
+  auto sparse = [&](int c, float x) {
+    float t = 0.f, g = 0.f;
+    if (soft) {
+#pragma unroll 4
+      for (int i = 0; i < a.k; ++i) {
+        const int2 e = s_e[i];
+        t += e.x == c ? __int_as_float(e.y) : 0.f;
+      }
+      g += w * (fs * __builtin_amdgcn_exp2f(fmaf(x, c1, b1)) - soft_w * a.tau * t);
+    }
+    if (has_y) g += w * (fh * __builtin_amdgcn_exp2f(TWO ? fmaf(x, LOG2E, b2) : fmaf(x, c1, b1)) - (c == (int)y ? a.hard : 0.f));
+    return P::store(g);
+  };
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // the dense values are written: a store behind the barrier to the same place comes second
+  __syncthreads();
+  if (soft) {
+#pragma unroll 1
+    for (int j = tid; j < a.k; j += NT)
+      if (s_e[j].x >= 0) dz[s_e[j].x] = sparse(s_e[j].x, s_z[j]);
+  }
+  if (has_y && tid == NT - 1) dz[y] = sparse((int)y, zy);
 }
 
 template <typename T>
