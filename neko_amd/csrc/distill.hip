@@ -98,7 +98,7 @@ template <> struct Piece<float> {
 // maximum, 7 (13 with TWO) for the sums, 7.5 (12.5) for the gradient, an exponential counting four.
 // two workgroups of 1024 per CU where the row leaves room (64 registers): one loads while the other computes
 template <typename T, int NT, int NCH, bool TWO>
-__global__ __launch_bounds__(NT, NCH <= 7 ? 8 : 4) void distill_kernel(DistillArgs a) {
+__global__ __launch_bounds__(NT, NCH <= 7 ? 8 : NT == 512 ? 6 : 4) void distill_kernel(DistillArgs a) {
   using P = Piece<T>;
   constexpr int N = P::N, NW = NT / 64;
   constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
@@ -340,7 +340,7 @@ int launch(const DistillArgs& a, int R, hipStream_t s) {
   if (nch <= 256) NEKO_DISTILL(256, 1);                 // short vocabularies: small workgroups, several rows per CU
   else if (nch <= 1024) NEKO_DISTILL(256, 4);
   else if (nch <= 4 * 1024) NEKO_DISTILL(1024, 4);
-  else if (nch <= 7 * 1024) NEKO_DISTILL(1024, 7);
+  else if (nch <= 7 * 1024) NEKO_DISTILL(512, 14);
   else if (nch <= 13 * 1024) NEKO_DISTILL(1024, 13);
   else NEKO_DISTILL(1024, 0);
 #undef NEKO_DISTILL
