@@ -458,44 +458,63 @@ class KVDecoder:
     caller resets and re-primes on the truncated window (same semantics, see GatoPolicy._decode_tokens)."""
 
     def __init__(self, P: StackParams, cap: int, device):
-        self.P, self.cap, self.n = P, int(cap), 0
+        self.P, self.cap, self.n, self.device = P, int(cap), 0, device
         self.qkv = [torch.zeros(self.cap, 3 * P.d, dtype=BF16, device=device) for _ in P.layers]
         self.kbias = torch.zeros(1, self.cap, dtype=F32, device=device)       # all positions real: no key bias
         self.kstart = torch.zeros(1, dtype=torch.int32, device=device)
         self.pos = torch.zeros(1, dtype=torch.int32, device=device)           # device-side index of the next row
         self.fast_row = P.d % 8 == 0 and 4 * P.d <= 3072                      # neko_gemv_bf16 limits (K <= 3072)
 
+    few_rows = 1             # most rows _few_rows takes (its attention reads their position from device memory)
+
     def reset(self) -> None:
         self.n = 0
         self.pos.zero_()
 
+    def truncate(self, n: int) -> None:
+        """Forget every position from n on (drafted tokens that were not kept): later rows overwrite them."""
+        assert 0 <= n <= self.n, f"truncate({n}) of {self.n} positions"
+        self.n = n
+        self.pos.fill_(n)
+
+    def _attend_few(self, li: int, rows: torch.Tensor, o: torch.Tensor) -> None:
+        """o (n, d) <- attention of the newest n <= few_rows q|k|v rows at *pos; appends their keys and values."""
+        P = self.P
+        ops.attn_decode(self.qkv[li], rows, self.pos, o, P.heads, P.d // P.heads)
+
+    def _project_attend(self, li: int, lp: LayerParams, a1: torch.Tensor, n0: int, T: int) -> torch.Tensor:
+        """Any number of new rows (positions n0 .. T-1): projection into the cache, attention over it -> o (T - n0, d)."""
+        d, H = self.P.d, self.P.heads
+        ops.gemm(a1, lp.w_qkv, T - n0, 3 * d, d, b_kstrided=True, bias=lp.b_qkv, out_bf16=self.qkv[li][n0:T], ldcb=3 * d)
+        o_all, _ = ops.attn_fwd(self.qkv[li][:T], self.kbias[:, :T].contiguous(), self.kstart, 1, T, H, d // H)
+        return o_all[n0:T]
+
     # ---- single-row step with a device-side position (HIP-graph capturable) -------------------------------------
-    def _one_row(self, x: torch.Tensor) -> torch.Tensor:
-        """x (1, d) fp32 at position *self.pos -> ln_f(hidden) (1, d) bf16.  No host-side shape depends on the position
+    def _few_rows(self, x: torch.Tensor) -> torch.Tensor:
+        """x (n <= few_rows, d) fp32 at positions *self.pos .. -> ln_f(hidden) (n, d) bf16.  No host-side shape depends on the position
         (the attention call reads it from device memory), so this body can be captured once; the products are weight
         streams (neko_gemv_bf16), not tiled GEMMs."""
         P = self.P
-        d, H = P.d, P.heads
-        hd = d // H
+        d, n = P.d, x.shape[0]
         dev = x.device
         for li, lp in enumerate(P.layers):
-            a1 = torch.empty(1, d, dtype=BF16, device=dev)
+            a1 = torch.empty(n, d, dtype=BF16, device=dev)
             ops.layernorm_fwd(x, lp.ln1_w, lp.ln1_b, y16=a1, eps=P.eps)
-            row = torch.empty(1, 3 * d, dtype=BF16, device=dev)
-            ops.gemv(a1, lp.w_qkv, 1, 3 * d, d, b_kstrided=True, bias=lp.b_qkv, out_bf16=row)
-            o = torch.empty(1, d, dtype=BF16, device=dev)
-            ops.attn_decode(self.qkv[li], row, self.pos, o, H, hd)
-            x1 = torch.empty(1, d, dtype=F32, device=dev)
-            ops.gemv(o, lp.w_o, 1, d, d, b_kstrided=True, bias=lp.b_o, resid=x, out_f32=x1)
-            a2 = torch.empty(1, d, dtype=BF16, device=dev)
+            row = torch.empty(n, 3 * d, dtype=BF16, device=dev)
+            ops.gemv(a1, lp.w_qkv, n, 3 * d, d, b_kstrided=True, bias=lp.b_qkv, out_bf16=row)
+            o = torch.empty(n, d, dtype=BF16, device=dev)
+            self._attend_few(li, row, o)
+            x1 = torch.empty(n, d, dtype=F32, device=dev)
+            ops.gemv(o, lp.w_o, n, d, d, b_kstrided=True, bias=lp.b_o, resid=x, out_f32=x1)
+            a2 = torch.empty(n, d, dtype=BF16, device=dev)
             ops.layernorm_fwd(x1, lp.ln2_w, lp.ln2_b, y16=a2, eps=P.eps)
-            h = torch.empty(1, 4 * d, dtype=BF16, device=dev)
-            ops.gemv(a2, lp.w_fc, 1, 4 * d, d, b_kstrided=True, bias=lp.b_fc, act=1, out_bf16=h)
-            _geglu_gate(lp, a2, h, 1, d)
-            x2 = torch.empty(1, d, dtype=F32, device=dev)
-            ops.gemv(h, lp.w_pr, 1, d, 4 * d, b_kstrided=True, bias=lp.b_pr, resid=x1, out_f32=x2)
+            h = torch.empty(n, 4 * d, dtype=BF16, device=dev)
+            ops.gemv(a2, lp.w_fc, n, 4 * d, d, b_kstrided=True, bias=lp.b_fc, act=1, out_bf16=h)
+            _geglu_gate(lp, a2, h, n, d)
+            x2 = torch.empty(n, d, dtype=F32, device=dev)
+            ops.gemv(h, lp.w_pr, n, d, 4 * d, b_kstrided=True, bias=lp.b_pr, resid=x1, out_f32=x2)
             x = x2
-        hf16 = torch.empty(1, d, dtype=BF16, device=dev)
+        hf16 = torch.empty(n, d, dtype=BF16, device=dev)
         ops.layernorm_fwd(x, P.lnf_w, P.lnf_b, y16=hf16, eps=P.eps)
         return hf16
 
@@ -505,13 +524,13 @@ class KVDecoder:
         At B = 1 a step is ~70 launches and launch-bound; replaying the graph costs one.  Call before priming (the
         warm-up runs write cache row 0, which the prime overwrites)."""
         d = self.P.d
-        dev = self.qkv[0].device
+        dev = self.pos.device
         self.g_x = torch.zeros(1, d, dtype=F32, device=dev)
         self.g_logits = torch.zeros(end - start + 1, dtype=F32, device=dev)
         self.g_token = torch.zeros((), dtype=torch.int64, device=dev)
 
         def body():
-            h = self._one_row(self.g_x)
+            h = self._few_rows(self.g_x)
             lg = lm_head_rows(Hp, h)[0, start:(end + 1)]
             tok = torch.argmax(lg, dim=-1) + start
             self.g_logits.copy_(lg)
@@ -545,25 +564,21 @@ class KVDecoder:
     def extend(self, x_new: torch.Tensor) -> torch.Tensor:
         """x_new (n, d) fp32 embeddings of the next n positions -> ln_f(hidden) of those positions, bf16 (n, d)."""
         P = self.P
-        d, H = P.d, P.heads
-        hd = d // H
+        d = P.d
         x = x_new.reshape(-1, d).to(F32).contiguous()
         n, dev = x.shape[0], x.device
         n0, T = self.n, self.n + n
         if T > self.cap:
             raise ValueError(f"KVDecoder: {T} positions exceed the capacity {self.cap}")
-        if n == 1 and self.fast_row:                # the decode step proper: weight-streaming products, 1-query attention
-            hf16 = self._one_row(x)                 # reads / appends at *pos == n0
+        if n <= self.few_rows and self.fast_row:    # the decode step proper: weight-streaming products, few-query attention
+            hf16 = self._few_rows(x)                # reads / appends at *pos == n0
             self.n = T
             self.pos.fill_(T)
             return hf16
-        kb = self.kbias[:, :T].contiguous()
         for li, lp in enumerate(P.layers):
             a1 = torch.empty(n, d, dtype=BF16, device=dev)
             ops.layernorm_fwd(x, lp.ln1_w, lp.ln1_b, y16=a1, eps=P.eps)
-            ops.gemm(a1, lp.w_qkv, n, 3 * d, d, b_kstrided=True, bias=lp.b_qkv, out_bf16=self.qkv[li][n0:T], ldcb=3 * d)
-            o_all, _ = ops.attn_fwd(self.qkv[li][:T], kb, self.kstart, 1, T, H, hd)
-            o = o_all[n0:T]
+            o = self._project_attend(li, lp, a1, n0, T)
             x1 = torch.empty(n, d, dtype=F32, device=dev)
             ops.gemm(o, lp.w_o, n, d, d, b_kstrided=True, bias=lp.b_o, resid=x, out_f32=x1)
             a2 = torch.empty(n, d, dtype=BF16, device=dev)
@@ -579,6 +594,37 @@ class KVDecoder:
         self.n = T
         self.pos.fill_(T)                           # device-side position of the next row
         return hf16
+
+
+class KV8Decoder(KVDecoder):
+    """KVDecoder over an 8-bit cache (ops.KV8Cache: e4m3 or int8, a scale per block of positions and head): half the bytes of the bf16 rows'
+    keys and values.  Up to eight new rows at a time take the weight-streaming step (a decode step, or the drafted tokens of a verification),
+    longer extensions attend to the cache instead of recomputing every row.  window > 0: a row sees the last `window` positions and the first
+    `sinks`, so a sequence may run past the context without recomputing it (the cache then holds `cap` positions, whatever the window)."""
+
+    few_rows = 8
+
+    def __init__(self, P: StackParams, cap: int, device, dtype=torch.float8_e4m3fn, block: int = 32, window: int = 0, sinks: int = 0):
+        self.P, self.cap, self.n, self.device = P, int(cap), 0, device
+        self.window, self.sinks = int(window), int(sinks)
+        size = (self.cap + 63) // 64 * 64
+        self.caches = [ops.KV8Cache(1, P.heads, size, P.d // P.heads, dtype=dtype, block=block, device=device) for _ in P.layers]
+        self.pos = torch.zeros(1, dtype=torch.int32, device=device)           # device-side index of the next row
+        self.fast_row = P.d % 8 == 0 and 4 * P.d <= 3072                      # neko_gemv_bf16 limits (K <= 3072)
+
+    def _attend_few(self, li: int, rows: torch.Tensor, o: torch.Tensor) -> None:
+        H, c = self.P.heads, self.caches[li]
+        x = rows.view(1, rows.shape[0], 3, H, c.hd)
+        ops.kv8_append(c, x[:, :, 1], x[:, :, 2], self.pos)
+        ops.attn_kv8(c, x[:, :, 0], self.pos, window=self.window, sinks=self.sinks, out=o.view(1, rows.shape[0], H, c.hd))
+
+    def _project_attend(self, li: int, lp: LayerParams, a1: torch.Tensor, n0: int, T: int) -> torch.Tensor:
+        d, n = self.P.d, T - n0
+        qkv = torch.empty(n, 3 * d, dtype=BF16, device=a1.device)
+        ops.gemm(a1, lp.w_qkv, n, 3 * d, d, b_kstrided=True, bias=lp.b_qkv, out_bf16=qkv)
+        o = torch.empty(n, d, dtype=BF16, device=a1.device)
+        self._attend_few(li, qkv, o)
+        return o
 
 
 def lm_head_rows(Hp: HeadParams, h16: torch.Tensor) -> torch.Tensor:
@@ -612,8 +658,18 @@ def lm_head_logits(Hp: HeadParams, hf16: torch.Tensor) -> torch.Tensor:
     return logits
 
 
+@dataclass
+class Teacher:
+    """What a student is distilled from: the k top logits of a teacher at every loss row of the batch (in packed order) and their token
+    ids.  The row's loss is (1 - hard) tau^2 KL(teacher || student at tau) + hard * cross-entropy with the label (ops.distill_topk)."""
+    values: torch.Tensor          # fp32 [n_loss, k]
+    indices: torch.Tensor         # int32 [n_loss, k], -1: no entry
+    tau: float = 1.0
+    hard: float = 0.0
+
+
 def lm_head_loss(Hp: HeadParams, hf16: torch.Tensor, target: torch.Tensor, sel: Optional[torch.Tensor], count: Optional[torch.Tensor],
-                 want_grad: bool, chunk_rows: int = 4096, weight: Optional[torch.Tensor] = None):
+                 want_grad: bool, chunk_rows: int = 4096, weight: Optional[torch.Tensor] = None, teacher: Optional[Teacher] = None):
     """Chunked LM head + CE.  Never materialises (B,T,V) fp32 logits nor the (N,V) gathered copy
     (gato_policy.py:184-185): per chunk of rows it runs logits GEMM -> CE (loss rows + bf16 dlogits).
     Returns (loss scalar tensor, dlogits bf16 [M,Vpad] | None)."""
@@ -633,6 +689,10 @@ def lm_head_loss(Hp: HeadParams, hf16: torch.Tensor, target: torch.Tensor, sel: 
         # N = Vpad, not V: the padded rows of the table are zero, the CE kernel masks columns >= V, and every tile is
         # then an interior tile with 16-B aligned rows (fast GEMM epilogue)
         ops.gemm(hf16[r0:r1], Hp.w, n, Hp.Vpad, d, ldb=d, out_bf16=z, ldcb=Hp.Vpad)
+        if teacher is not None:
+            ops.distill_topk(z, Hp.V, Hp.Vpad, teacher.values[r0:r1], teacher.indices[r0:r1], weight[r0:r1], tau=teacher.tau, target=target[r0:r1],
+                             hard=teacher.hard, loss_row=loss_rows[r0:r1], dlogits=z if want_grad else None)
+            continue
         ops.ce_bf16_inplace(z, Hp.V, Hp.Vpad, target[r0:r1], weight[r0:r1], loss_row=loss_rows[r0:r1],
                             want_grad=want_grad)
     loss = (loss_rows * weight).sum()       # (not torch.dot: a BLAS call inside a captured step)
@@ -662,7 +722,7 @@ def _selected_weight(n: int, npad: int, dev) -> torch.Tensor:
 
 def lm_head_loss_selected(Hp: HeadParams, hf16: torch.Tensor, target: Optional[torch.Tensor], idx: torch.Tensor, n: int,
                           want_grad: bool, chunk_rows: int = 4096, tokens_flat: Optional[torch.Tensor] = None,
-                          tgt_idx: Optional[torch.Tensor] = None):
+                          tgt_idx: Optional[torch.Tensor] = None, teacher: Optional[Teacher] = None):
     """Same loss as lm_head_loss, but only the n selected positions (idx: int32 flat row indices, known on the
     host from the packing descriptors) go through the LM head -- the HIP counterpart of the reference's
     boolean-mask gather (gato_policy.py:183-185), done before the GEMM instead of after it.
@@ -679,7 +739,10 @@ def lm_head_loss_selected(Hp: HeadParams, hf16: torch.Tensor, target: Optional[t
         torch.index_select(tokens_flat, 0, tgt_idx[:n], out=tsel[:n])
     else:
         tsel[:n] = target.index_select(0, idx[:n].long())
-    loss, dlogits = lm_head_loss(Hp, hsel, tsel, None, None, want_grad, chunk_rows, weight=_selected_weight(n, npad, dev))
+    if teacher is not None and npad > n:            # the padding rows weigh 0: their teacher is never looked at
+        pad = torch.nn.functional.pad
+        teacher = Teacher(pad(teacher.values, (0, 0, 0, npad - n)), pad(teacher.indices, (0, 0, 0, npad - n), value=-1), teacher.tau, teacher.hard)
+    loss, dlogits = lm_head_loss(Hp, hsel, tsel, None, None, want_grad, chunk_rows, weight=_selected_weight(n, npad, dev), teacher=teacher)
     return loss, hsel, dlogits
 
 

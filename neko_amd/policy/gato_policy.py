@@ -297,10 +297,11 @@ class _PolicyCoreFn(torch.autograd.Function):
     """packed embeddings -> (logits | empty, loss | empty): transformer stack + LM head + masked CE."""
 
     @staticmethod
-    def forward(ctx, policy: "GatoPolicy", x, pmask, tokens, tmask, compute_loss: bool, return_logits: bool, pack, *params):
+    def forward(ctx, policy: "GatoPolicy", x, pmask, tokens, tmask, compute_loss: bool, return_logits: bool, pack, teacher, *params):
         """pack: the `_PackInfo` of the `_tokenize` call that produced (x, tokens, tmask, pmask) in THIS forward, or None
         when the caller handed the four tensors in (kwargs form, gato_policy.py:161-165): the loss positions are then
-        derived from the masks that were passed, as the reference does (:176-183)."""
+        derived from the masks that were passed, as the reference does (:176-183).
+        teacher: engine.Teacher (the loss is then the distillation loss over the loss rows) or None."""
         need = bool(compute_loss) and any(ctx.needs_input_grad)   # grad mode is off inside Function.forward
         f = policy._flat
         f.ensure_shadow()
@@ -322,7 +323,8 @@ class _PolicyCoreFn(torch.autograd.Function):
                 target = None if pack.tgt_idx is not None else engine.shift_targets(tokens, tmask, pmask)[0]
                 loss, hf16, dlogits = engine.lm_head_loss_selected(hp, hf16, target, idx, n, want_grad=need,
                                                                    chunk_rows=policy.lm_head_chunk_rows,
-                                                                   tokens_flat=tokens.reshape(-1), tgt_idx=pack.tgt_idx)
+                                                                   tokens_flat=tokens.reshape(-1), tgt_idx=pack.tgt_idx,
+                                                                   teacher=teacher)
                 ctx.sel_idx, ctx.sel_n, ctx.sel_map = idx, n, pack.row_map
             else:
                 target, sel, count = engine.shift_targets(tokens, tmask, pmask)
@@ -527,6 +529,11 @@ class GatoPolicy(nn.Module):
         #: 0 = the reference's layout.  Same loss and gradients, fewer padded positions through the stack.
         self.ragged_groups = int(os.environ.get("NEKO_RAGGED_GROUPS", "0"))
         self.last_pack: Optional[_PackInfo] = None      # statistics of the last packed batch (bench / logging only)
+        #: what the decode helpers keep keys and values in: "bf16", or "e4m3" / "int8" with a scale per 32 positions and head (engine.KV8Decoder)
+        self.kv_cache = os.environ.get("NEKO_KV_CACHE", "bf16")
+        #: > 0 (8-bit caches only): a decoded row sees the last decode_window positions and the first decode_sinks, and a sequence that outgrows
+        #: context_len goes on instead of being cut on the left and recomputed
+        self.decode_window, self.decode_sinks = 0, 0
         self._dp = None
         self._layout_cache: "OrderedDict" = OrderedDict()      # structural memo of _prepare (layout_signature)
         self._hp = None
@@ -713,17 +720,23 @@ class GatoPolicy(nn.Module):
         x, tokens, tmask, pmask, pack = self._embed_prepared(pr)
         names = self.transformer._param_names() + ["predict_token.weight"]
         params = [self._flat.param_of[n] for n in names]
-        _, loss = _PolicyCoreFn.apply(self, x, pmask.to(torch.float32), tokens, tmask, True, False, pack, *params)
+        _, loss = _PolicyCoreFn.apply(self, x, pmask.to(torch.float32), tokens, tmask, True, False, pack, None, *params)
         return loss
 
     # ---- forward (gato_policy.py:156-192) -------------------------------------------------------------
     def forward(self, inputs: Optional[list] = None, compute_loss=False, **kwargs):
         return_logits = kwargs.pop("return_logits", True)
+        teacher: Optional[engine.Teacher] = kwargs.pop("teacher", None)
+        if teacher is not None and not (inputs is not None and compute_loss and self.lm_head_selected_rows):
+            raise ValueError("teacher= needs inputs and compute_loss=True (its rows are the loss rows of the packed batch)")
         if inputs is not None:
             # length-bucketed layout: only when no (B, T, V) logits tensor has to be handed back (the training call,
             # trainer.py:178 discards them) -- the loss and every gradient are those of the padded layout
-            ragged = self.ragged_groups if (compute_loss and not return_logits and len(inputs) > 1) else 0
+            # (a teacher's rows are in the order of the plain layout, see top_logits)
+            ragged = self.ragged_groups if (compute_loss and not return_logits and len(inputs) > 1 and teacher is None) else 0
             token_embeddings, tokens, token_target_masks, token_masks, pack = self._tokenize(inputs, ragged)
+            if teacher is not None and (tuple(teacher.values.shape[:1]) != (pack.n_loss,) or pack.n_loss == 0):
+                raise ValueError(f"the batch has {pack.n_loss} loss rows, the teacher {tuple(teacher.values.shape)} logits")
         else:
             pack = None
             assert ("token_embeddings" in kwargs and "tokens" in kwargs and "token_target_masks" in kwargs
@@ -739,8 +752,22 @@ class GatoPolicy(nn.Module):
         names = self.transformer._param_names() + ["predict_token.weight"]
         params = [self._flat.param_of[n] for n in names]
         logits, loss = _PolicyCoreFn.apply(self, token_embeddings, token_masks.to(torch.float32), tokens,
-                                           token_target_masks, bool(compute_loss), bool(return_logits), pack, *params)
+                                           token_target_masks, bool(compute_loss), bool(return_logits), pack, teacher, *params)
         return (logits if return_logits else None), (loss if compute_loss else None)
+
+    @torch.no_grad()
+    def top_logits(self, inputs: list, k: int, tau: float = 1.0, hard: float = 0.0) -> engine.Teacher:
+        """This policy as a teacher: its k largest logits at every loss row of the batch, for `student.forward(inputs, compute_loss=True,
+        teacher=...)` on the same batch.  The LM head runs on the loss rows only, 4096 at a time."""
+        x, _, _, pmask, pack = self._tokenize(inputs, 0)
+        if pack.n_loss == 0:
+            raise ValueError("the batch has no loss rows")
+        self._flat.ensure_shadow()
+        hf16, _, _ = engine.stack_forward(self.transformer._stack_params(), x.to(torch.float32), pmask, save=False)
+        h = ops.gather_rows_bf16(hf16, pack.loss_idx, pack.n_loss, pack.n_loss)
+        tops = [torch.topk(engine.lm_head_rows(self._head_params(), h[r:r + 4096]), k, dim=1) for r in range(0, pack.n_loss, 4096)]
+        return engine.Teacher(torch.cat([t.values for t in tops]).contiguous(), torch.cat([t.indices for t in tops]).to(torch.int32).contiguous(),
+                              float(tau), float(hard))
 
     # ---- inference helpers (gato_policy.py:434-470, 477-544, 556-614) ----------------------------------------------
     # KV-cached decode (SURVEY.md 8(f) rank 2).  The reference re-runs the whole forward for every generated token;
@@ -749,6 +776,17 @@ class GatoPolicy(nn.Module):
     # window is truncated on the left and RE-PRIMED (every remaining row recomputed without the dropped ones, exactly
     # what a full forward over the truncated window computes).  Pinned by fixture G12 (tests/golden/
     # make_fixture_decode.py: the reference's own predict_text / predict_response / predict_control outputs).
+    def _new_decoder(self, cap: int, device) -> "engine.KVDecoder":
+        sp = self.transformer._stack_params()
+        if self.kv_cache == "bf16":
+            if self.decode_window:
+                raise ValueError("decode_window needs kv_cache = 'e4m3' or 'int8'")
+            return engine.KVDecoder(sp, cap, device)
+        kinds = {"e4m3": torch.float8_e4m3fn, "int8": torch.int8}
+        if self.kv_cache not in kinds:
+            raise ValueError(f"kv_cache must be 'bf16', 'e4m3' or 'int8', got {self.kv_cache!r}")
+        return engine.KV8Decoder(sp, cap, device, dtype=kinds[self.kv_cache], window=self.decode_window, sinks=self.decode_sinks)
+
     def _decode_tokens(self, token_embeddings, n_tokens, start_token, end_token, deterministic):
         """Autoregressive continuation of ONE unpadded sequence.  Returns (logits (n_tokens, end-start+1) fp32,
         list of 0-d token tensors in the global vocabulary)."""
@@ -757,7 +795,9 @@ class GatoPolicy(nn.Module):
         hp = self._head_params()
         self._flat.ensure_shadow()
         table = self._flat.view("embed_token.weight")
-        use_graph = (deterministic and n_tokens > 1 and emb.shape[0] + n_tokens - 1 <= self.context_len
+        # windowed decoding never recomputes: the cache holds every position instead
+        cap = self.context_len if not self.decode_window else max(self.context_len, (emb.shape[0] + n_tokens + 63) // 64 * 64)
+        use_graph = (deterministic and n_tokens > 1 and emb.shape[0] + n_tokens - 1 <= cap
                      and os.environ.get("NEKO_DECODE_GRAPH", "1") != "0")
         # decoders (cache buffers + the captured step) are kept per token range: capture costs ~100 ms, a rollout calls
         # this thousands of times.  The graph holds pointers into the flat parameter storage and its bf16 shadow, which
@@ -765,9 +805,11 @@ class GatoPolicy(nn.Module):
         if not hasattr(self, "_decoders"):
             self._decoders = {}
         key = (start_token, end_token) if use_graph else None
+        if self.kv_cache != "bf16":
+            key = (key, self.kv_cache, self.decode_window, self.decode_sinks)
         dec = self._decoders.get(key)
-        if dec is None:
-            dec = engine.KVDecoder(self.transformer._stack_params(), self.context_len, emb.device)
+        if dec is None or dec.cap < cap:
+            dec = self._new_decoder(cap, emb.device)
             if use_graph:
                 dec.capture_greedy_step(hp, table, start_token, end_token)
             self._decoders[key] = dec
@@ -798,7 +840,7 @@ class GatoPolicy(nn.Module):
             tokens.append(token)
             new = table[token].reshape(1, -1)
             emb = torch.cat([emb, new], dim=0)
-            if emb.shape[0] > self.context_len:           # window slides: reference semantics = recompute the window
+            if emb.shape[0] > cap:                        # window slides: reference semantics = recompute the window
                 emb = emb[-self.context_len:]
                 dec.reset()
                 h = dec.extend(emb)
@@ -811,6 +853,73 @@ class GatoPolicy(nn.Module):
         start_token, end_token = self.token_starts["text"], self.token_ends["text"]
         token_embeddings, _, _, _ = self.tokenize_input_dicts([batch_dict])
         return self._decode_tokens(token_embeddings, max_length, start_token, end_token, deterministic)
+
+    @torch.no_grad()
+    def predict_text_speculative(self, batch_dict, draft: "GatoPolicy", max_length=20, deterministic=True, n_draft=4, temperature=1.0, generator=None):
+        """predict_text with `draft` -- a smaller policy over the same vocabulary -- proposing n_draft tokens at a time and this policy judging them
+        in one step of n_draft + 1 rows (ops.verify_draft): greedy, the tokens are this policy's own best ones; sampled, they follow its
+        softmax at `temperature` exactly, whatever the draft proposes.  Same return value as predict_text.  Prompt, answer and drafts
+        have to fit in context_len (nothing is cut on the left here)."""
+        if not 1 <= n_draft <= 7:
+            raise ValueError("n_draft must be 1 .. 7 (a judging step takes up to 8 rows)")
+        if draft.vocab_size != self.vocab_size or draft.token_ends["text"] != self.token_ends["text"]:
+            raise ValueError("the drafting policy must have the same vocabulary")
+        if not deterministic and not temperature > 0:
+            raise ValueError("temperature must be positive")
+        lo, hi = self.token_starts["text"], self.token_ends["text"]
+        models = (self, draft)
+        embs = [m.tokenize_input_dicts([batch_dict])[0][0].to(torch.float32) for m in models]
+        for m, e in zip(models, embs):
+            if e.shape[0] + max_length + n_draft > m.context_len:
+                raise ValueError(f"{e.shape[0]} prompt positions, {max_length} tokens and {n_draft} drafts do not fit in context_len {m.context_len}")
+            m._flat.ensure_shadow()
+        tgt, drf = (m._new_decoder(m.context_len, m._dev()) for m in models)
+        tables = [m._flat.view("embed_token.weight") for m in models]
+        heads = [m._head_params() for m in models]
+        dev = self._dev()
+
+        def rows(which, h):
+            return engine.lm_head_rows(heads[which], h)[:, lo:hi + 1]
+
+        def pick(lg):           # (1, V) -> 0-d token within the text range
+            if deterministic:
+                return torch.argmax(lg[0])
+            return torch.multinomial(torch.softmax(lg[0] / temperature, -1), 1, generator=generator)[0]
+
+        first = rows(0, tgt.extend(embs[0])[-1:])
+        drf.extend(embs[1])
+        tok = pick(first)
+        logits, tokens = [first[0]], [int(tok)]
+        feed = [tokens[0]]                                   # what the draft has not seen yet
+        while len(tokens) < max_length:
+            proposed, dl = [], []
+            nxt = torch.tensor(feed, device=dev)
+            base_t, base_d = tgt.n, drf.n + len(feed)
+            for _ in range(n_draft):
+                lg = rows(1, drf.extend(tables[1].index_select(0, nxt + lo))[-1:])
+                nxt = pick(lg).reshape(1)
+                proposed.append(nxt)
+                dl.append(lg)
+            x = torch.cat(proposed)
+            judged = torch.cat([torch.tensor(tokens[-1:], device=dev), x])
+            lt = rows(0, tgt.extend(tables[0].index_select(0, judged + lo)))             # row i: the distribution of proposed token i
+            if deterministic:
+                acc, out = ops.verify_draft(lt.unsqueeze(0), x.reshape(1, -1), temperature=0.0)
+            else:
+                u = torch.rand((1, n_draft), device=dev, generator=generator)
+                r = torch.rand(1, device=dev, generator=generator)
+                acc, out = ops.verify_draft(lt.unsqueeze(0), x.reshape(1, -1), draft_logits=torch.cat(dl).unsqueeze(0), u=u, r=r, temperature=temperature)
+            new = [t for t in out[0].tolist() if t >= 0]         # the kept drafts and the token behind them (the step's one host read)
+            kept = len(new) - 1
+            logits += [lt[i] for i in range(len(new))]
+            tgt.truncate(base_t + 1 + kept)                  # the judged row and the kept drafts
+            if kept == n_draft:                              # the draft has not seen its own last token
+                feed = [new[kept - 1], new[kept]]
+            else:
+                drf.truncate(base_d + kept)
+                feed = [new[kept]]
+            tokens += new
+        return torch.stack(logits[:max_length]), [torch.tensor(t + lo, device=dev) for t in tokens[:max_length]]
 
     @torch.no_grad()
     def predict_response(self, image, prompt_tokens=[], max_length=128, deterministic=True):
@@ -826,7 +935,7 @@ class GatoPolicy(nn.Module):
         the embedding row of the newly chosen token, taken from the packing kernels (token + local position embedding)
         so the rows are the very ones the full forward would see."""
         dev = self._dev()
-        dec = engine.KVDecoder(self.transformer._stack_params(), self.context_len, dev)
+        dec = self._new_decoder(self.context_len, dev)
         hp = self._head_params()
         self._flat.ensure_shadow()
         n_patches = image_embeddings.shape[1]
