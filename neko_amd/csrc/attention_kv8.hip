@@ -30,32 +30,29 @@ struct Span {
   int pfirst;        // first position of the tile's rows
   int a0, na, b0, nt;
 };
-__device__ __forceinline__ bool span_of(const AttnArgs& a, int s, int r0, int r1, Span& sp) {
-  const int p = a.pos[s];
-  int n = min(a.n_new ? a.n_new[s] : a.T, a.T);
-  if (p < 0 || p >= a.cap || n <= 0) return false;
-  n = min(n, a.cap - p);
-  sp.rows = n * a.G;
-  if (r0 >= sp.rows) return false;
+__device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
+// (rows == 0: this row tile has nothing to do.  Every field is wave-uniform and in a scalar register: as a plain struct the compiler kept it in
+// scratch, and the reload of a field inside the key loop waited for the whole prefetch)
+__device__ __forceinline__ Span span_of(const AttnArgs& a, int s, int r0, int r1) {
+  const int p = uni(a.pos[s]);
+  const int given = a.n_new ? uni(a.n_new[s]) : a.T;
+  const bool ok = p >= 0 && p < a.cap && given > 0;
+  const int n = ok ? min(min(given, a.T), a.cap - p) : 0;
+  Span sp;
+  sp.rows = r0 < n * a.G ? n * a.G : 0;
   sp.p0 = p;
   sp.pfirst = p + r0 / a.G;
-  sp.plast = p + (min(r1, sp.rows) - 1) / a.G;
-  sp.first = a.start ? max(a.start[s], 0) : 0;
-  if (sp.first > sp.plast) { sp.a0 = sp.na = sp.b0 = sp.nt = 0; return true; }
-  int lo = sp.first;
-  if (a.window > 0 && sp.pfirst - a.window + 1 > lo) lo = sp.pfirst - a.window + 1;
+  sp.plast = p + max(min(r1, n * a.G) - 1, 0) / a.G;
+  sp.first = a.start ? max(uni(a.start[s]), 0) : 0;
+  const int lo = a.window > 0 ? max(sp.first, sp.pfirst - a.window + 1) : sp.first;
+  const int sink_last = (int)min((long)sp.first + a.sinks - 1, (long)sp.plast);
   sp.b0 = lo >> 6;
-  const int nb = (sp.plast >> 6) + 1 - sp.b0;
   sp.a0 = sp.first >> 6;
-  sp.na = 0;
-  if (a.window > 0 && a.sinks > 0) {
-    const int sink_last = (int)min((long)sp.first + a.sinks - 1, (long)sp.plast);
-    sp.na = max(0, min((sink_last >> 6) + 1, sp.b0) - sp.a0);
-  }
-  sp.nt = sp.na + nb;
-  return true;
+  sp.na = a.window > 0 && a.sinks > 0 ? max(0, min((sink_last >> 6) + 1, sp.b0) - sp.a0) : 0;
+  sp.nt = sp.first > sp.plast ? 0 : sp.na + (sp.plast >> 6) + 1 - sp.b0;
+  return sp;
 }
-__device__ __forceinline__ int tile_of(const Span& sp, int i) { return i < sp.na ? sp.a0 + i : sp.b0 + i - sp.na; }
+__device__ __forceinline__ int tile_of(const Span& sp, int i) { return i + (i < sp.na ? sp.a0 : sp.b0 - sp.na); }
 __device__ __forceinline__ bool visible(const AttnArgs& a, const Span& sp, int key, int p) {
   return key <= p && key >= sp.first && (a.window == 0 || key > p - a.window || key < (long)sp.first + a.sinks);
 }
@@ -76,12 +73,12 @@ __global__ __launch_bounds__(NW * 64, NQ == 1 || (NQ == 2 && HD < 128) ? 2 : 1) 
   constexpr int LDO = HD + 4;
   __shared__ float sm_o[NW][16][LDO];
   __shared__ float sm_ml[NW][16][2];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4;
   const int split = blockIdx.x % a.splits, rt = blockIdx.x / a.splits;
   const int h = blockIdx.y, s = blockIdx.z;
-  Span sp;
-  if (!span_of(a, s, rt * NQ * 16, rt * NQ * 16 + NQ * 16, sp)) return;
+  const Span sp = span_of(a, s, rt * NQ * 16, rt * NQ * 16 + NQ * 16);
+  if (sp.rows == 0) return;
   const int per = (sp.nt + a.splits - 1) / a.splits;
   const int i_end = min(sp.nt, (split + 1) * per);
   const long head = (long)s * a.H + h;
@@ -309,13 +306,13 @@ __global__ __launch_bounds__(NW * 64) void attn_kv8_tile_kernel(AttnArgs a) {
   constexpr int NT = NW * 64;
   constexpr int UPT = (2 * UNITS + NT - 1) / NT;          // pieces per thread
   __shared__ __attribute__((aligned(16))) char smem[2][2 * IMG];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
   const int r = lane & 31, hf = lane >> 5;
   const int split = blockIdx.x % a.splits, rt = a.rtiles - 1 - blockIdx.x / a.splits;     // the row tiles with the most keys first
   const int h = blockIdx.y, s = blockIdx.z;
   constexpr int RT = NW * 32;
-  Span sp;
-  if (!span_of(a, s, rt * RT, rt * RT + RT, sp)) return;
+  const Span sp = span_of(a, s, rt * RT, rt * RT + RT);
+  if (sp.rows == 0) return;
   const int per = (sp.nt + a.splits - 1) / a.splits;
   const int i0 = split * per, i_end = min(sp.nt, i0 + per);
   const long head = (long)s * a.H + h;
