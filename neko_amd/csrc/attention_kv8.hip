@@ -6,8 +6,11 @@
 // Rows i >= n_new[s] are left as they are; a row that sees nothing is 0.  Codes are unpacked to bf16 (exact), scores, maxima, sums and the
 // output accumulate in fp32; block scales never touch an operand: K's multiplies the scores, V's the probabilities.
 #include "kv8.h"
+#include <type_traits>
 
 namespace {
+
+constexpr float NEVER = -3.0e38f;       // a running maximum before any visible key (finite: no special cases)
 
 struct AttnArgs {
   const uint8_t *k8, *v8;
@@ -323,6 +326,8 @@ __global__ __launch_bounds__(NW * 64) void attn_kv8_tile_kernel(AttnArgs a) {
 
   const int row = rt * RT + wave * 32 + r;
   const int w0 = rt * RT + wave * 32;                     // the wave's first row
+  // two waves share a SIMD (i and i + 4): the first goes ahead, so that its exponentials run beside the other's products
+  if (NW == 8 && wave < 4) __builtin_amdgcn_s_setprio(1);
   const bool wave_on = w0 < sp.rows;
   const int rc = min(row, sp.rows - 1);
   const int t = rc / a.G, gq = rc - t * a.G;
@@ -339,7 +344,10 @@ __global__ __launch_bounds__(NW * 64) void attn_kv8_tile_kernel(AttnArgs a) {
   for (int c = 0; c < NC; ++c)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[c][i] = 0.f;
-  float m = -INFINITY, l = 0.f;
+  float m = NEVER, l = 0.f;
+  // the queries are waited for here: left to the first product, that wait would stand in the key loop and cover the prefetch there too
+#pragma unroll
+  for (int k = 0; k < NK; ++k) asm volatile("" : "+v"(qf[k]));
 
   uint4 st[UPT];
   float ss[UPT];
@@ -356,7 +364,7 @@ __global__ __launch_bounds__(NW * 64) void attn_kv8_tile_kernel(AttnArgs a) {
     }
   };
   auto stage = [&](int tile, char* img) {
-    const bool edge = tile * KT < sp.first || tile * KT + KT - 1 > sp.plast;
+    const bool edge = tile * KT < sp.first || tile * KT + KT - 1 > sp.plast;      // positions out there hold whatever was left: zeros
 #pragma unroll
     for (int i = 0; i < UPT; ++i) {
       const int u = tid + i * NT;
@@ -372,11 +380,15 @@ __global__ __launch_bounds__(NW * 64) void attn_kv8_tile_kernel(AttnArgs a) {
         const int lr = (key & 32) + 8 * ((kk >> 2) & 3) + 4 * (kk >> 4) + (kk & 3);
         at0 = kimg<HD>(lr, 2 * cc);
         at1 = kimg<HD>(lr, 2 * cc + 1);
+        if (edge && (tile * KT + key < sp.first || tile * KT + key > sp.plast)) {
+          w[0] = w[1] = w[2] = w[3] = 0;
+          sc = 0.f;
+        }
       } else {
         const int t16 = uu / HD, ch = uu % HD;
         at0 = IMG + ((2 * t16) * HD + ch) * 16;
         at1 = at0 + HD * 16;
-        if (edge) {                                       // positions outside [first, plast] hold whatever was left there
+        if (edge) {
           const int lo = sp.first - (tile * KT + t16 * 16), hi = sp.plast - (tile * KT + t16 * 16);
 #pragma unroll
           for (int d = 0; d < 4; ++d) {
@@ -407,69 +419,78 @@ __global__ __launch_bounds__(NW * 64) void attn_kv8_tile_kernel(AttnArgs a) {
     if (more) fetch(tile_of(sp, it + 1));
     const int tk = tile * KT;
     if (wave_on && tk <= wlast) {
-      f32x16 sc[2];
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sc[kt][i] = 0.f;
-#pragma unroll
-      for (int k = 0; k < NK; ++k)
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-          const bf16x8_v kf = *reinterpret_cast<const bf16x8_v*>(img + kimg<HD>(kt * 32 + r, 2 * k + hf));
-          sc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[k], sc[kt], 0, 0, 0);
-        }
       const bool plain = tk >= sp.first && tk + KT - 1 <= wfirst && (a.window == 0 || tk > wlast - a.window);
-      if (!plain) {
+      f32x16 sc[2];
+      auto scores = [&]() {
+#pragma unroll
+        for (int k = 0; k < NK; ++k)
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt) {
+            const bf16x8_v kf = *reinterpret_cast<const bf16x8_v*>(img + kimg<HD>(kt * 32 + r, 2 * k + hf));
+            sc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[k], sc[kt], 0, 0, 0);
+          }
+        // operand reads run AHEAD products before their use (scheduled next to it, every product waited for its own read)
+        constexpr int AHEAD = 2 * NK < 6 ? 2 * NK : 6;
+        __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+        for (int i = 0; i < 2 * NK - AHEAD; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
+      };
+      // the mask is what the products start from, 0 or -inf (positions outside [first, plast] were zeroed on their way into LDS): the scores are
+      // written by the products alone and stay where those leave them
+      if (plain) {
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (!visible(a, sp, tk + kt * 32 + hf * 16 + i, prow)) sc[kt][i] = -INFINITY;
+          for (int i = 0; i < 16; ++i) sc[kt][i] = 0.f;
+        scores();
+      } else {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[kt][i] = visible(a, sp, tk + kt * 32 + hf * 16 + i, prow) ? 0.f : -INFINITY;
+        scores();
       }
-      float mx = sc[0][0];
+      {
+        float mx = sc[0][0];
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+        for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[kt][i]);
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * a.scale_log2e;        // scale > 0 (checked on entry)
-      if (__builtin_amdgcn_ballot_w64(mx > m + 8.0f || (m == -INFINITY && mx > m))) {
-        const float mn = fmaxf(m, mx);
-        const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
-        m = mn;
-        l *= alpha;
+          for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[kt][i]);
+        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+        mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * a.scale_log2e;        // scale > 0 (checked on entry)
+        if (__builtin_amdgcn_ballot_w64(mx > m + 8.0f)) {
+          const float mn = fmaxf(m, mx);
+          const float alpha = __builtin_amdgcn_exp2f(m - mn);
+          m = mn;
+          l *= alpha;
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
+          for (int c = 0; c < NC; ++c)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[c][i] *= alpha;
-      }
-      const float ms = m == -INFINITY ? 0.f : m;
-      float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[kt][i], a.scale_log2e, -ms)), p1 = __builtin_amdgcn_exp2f(fmaf(sc[kt][i + 1], a.scale_log2e, -ms));
-          sc[kt][i] = p0;
-          sc[kt][i + 1] = p1;
-          sum0 += p0;
-          sum1 += p1;
+            for (int i = 0; i < 16; ++i) o[c][i] *= alpha;
         }
-      l += sum0 + sum1;
+        float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+        for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          float y[8];
+          for (int u = 0; u < 2; ++u) {
+            float y[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = sc[kt][8 * u + e];
-          const bf16x8_v pf = pack8_bf16(y);
+            for (int e = 0; e < 8; ++e) y[e] = __builtin_amdgcn_exp2f(fmaf(sc[kt][8 * u + e], a.scale_log2e, -m));
 #pragma unroll
-          for (int c = 0; c < NC; ++c) {
-            const bf16x8_v vf = *reinterpret_cast<const bf16x8_v*>(img + IMG + ((kt * 4 + 2 * hf + u) * HD + c * 32 + r) * 16);
-            o[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf, o[c], 0, 0, 0);
+            for (int e = 0; e < 8; e += 2) { sum0 += y[e]; sum1 += y[e + 1]; }
+            const bf16x8_v pf = pack8_bf16(y);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+              const bf16x8_v vf = *reinterpret_cast<const bf16x8_v*>(img + IMG + ((kt * 4 + 2 * hf + u) * HD + c * 32 + r) * 16);
+              o[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf, o[c], 0, 0, 0);
+            }
           }
-        }
+        l += sum0 + sum1;
+      }
     }
     if (more) stage(tile_of(sp, it + 1), smem[(it + 1 - i0) & 1]);
     __syncthreads();
