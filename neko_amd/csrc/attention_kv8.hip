@@ -56,8 +56,13 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, int s, int r0, int r1
   return sp;
 }
 __device__ __forceinline__ int tile_of(const Span& sp, int i) { return i + (i < sp.na ? sp.a0 : sp.b0 - sp.na); }
-__device__ __forceinline__ bool visible(const AttnArgs& a, const Span& sp, int key, int p) {
-  return key <= p && key >= sp.first && (a.window == 0 || key > p - a.window || key < (long)sp.first + a.sinks);
+// the keys a row at position p sees: [first, p], without (lowest, sinks_end) if there is a window.  No short cuts: selects, no branches.
+struct Sight { int p, first, low, sinks_end; };
+__device__ __forceinline__ Sight sight_of(const AttnArgs& a, const Span& sp, int p) {
+  return Sight{p, sp.first, a.window > 0 ? p - a.window : -1, a.window > 0 ? (int)min((long)sp.first + a.sinks, 0x7fffffffL) : 0};
+}
+__device__ __forceinline__ bool visible(const Sight& v, int key) {
+  return (key <= v.p) & (key >= v.first) & ((key > v.low) | (key < v.sinks_end));
 }
 
 // ---- few rows: a wave owns whole key tiles --------------------------------------------------------------------------------
@@ -92,12 +97,12 @@ __global__ __launch_bounds__(NW * 64, NQ == 1 || (NQ == 2 && HD < 128) ? 2 : 1) 
 
   // queries: contraction slot (step, g, j) is channel 16 (4 (step / 2) + g) + 8 (step % 2) + j, for hd = 32 channel 8 g + j
   bf16x8_v qf[NQ][NK];
-  int prow[NQ];                               // position of the lane's row
+  Sight sight[NQ];                            // what the lane's row sees
 #pragma unroll
   for (int iq = 0; iq < NQ; ++iq) {
     const int row = min(rt * NQ * 16 + iq * 16 + r, sp.rows - 1);
     const int t = row / a.G, gq = row - t * a.G;
-    prow[iq] = sp.p0 + t;
+    sight[iq] = sight_of(a, sp, sp.p0 + t);
     const bf16_t* qp = a.q + a.q_ss * s + a.q_st * t + (long)(h * a.G + gq) * HD;
 #pragma unroll
     for (int k = 0; k < NK; ++k) {
@@ -184,7 +189,7 @@ __global__ __launch_bounds__(NW * 64, NQ == 1 || (NQ == 2 && HD < 128) ? 2 : 1) 
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           x[4 * t + i] = st[iq][t][i] * sc;
-          if (!plain) x[4 * t + i] = visible(a, sp, key0 + 4 * t + i, prow[iq]) ? x[4 * t + i] : -INFINITY;
+          if (!plain) x[4 * t + i] = visible(sight[iq], key0 + 4 * t + i) ? x[4 * t + i] : -INFINITY;
         }
       float mx = x[0];
 #pragma unroll
@@ -287,14 +292,19 @@ __global__ __launch_bounds__(NW * 64, NQ == 1 || (NQ == 2 && HD < 128) ? 2 : 1) 
 }
 
 // ---- many rows: key tiles through LDS -------------------------------------------------------------------------------------
-// One workgroup of NW waves per (split, head, sequence, row tile of 32 NW rows); a wave owns 32 rows.  A 64-key tile is unpacked ONCE, on
-// its way into LDS (codes x scale as bf16: exact), and read there by every wave as matrix operands; the codes of the tile after it are
-// loaded meanwhile, one barrier per tile.  32 x 32 x 16 products: S^T = K Q^T, then O^T = V^T P^T with the probabilities as they stand --
-// LDS row r of a 32-key half tile holds key 16 ((r >> 2) & 1) + 4 (r >> 3) + (r & 3), so that a lane's 16 scores are 16 consecutive keys.
+// One workgroup of NW waves per (split, head, sequence, row tile of 32 NW rows); a wave owns 32 rows.  A 64-key tile is unpacked ONCE, on its way
+// into LDS (codes x scale as bf16: exact), and read there by every wave as matrix operands; the codes of the tile after it are on their way
+// meanwhile, one barrier per tile.  32 x 32 x 16 products: S^T = K Q^T, then O^T = V^T P^T with the probabilities as they stand -- LDS row r of a
+// 32-key half tile holds key 16 ((r >> 2) & 1) + 4 (r >> 3) + (r & 3), so that a lane's 16 scores are 16 consecutive keys.
 //   K image: rows of HD bf16, 16-byte pieces XORed with the row (16 lanes read 16 rows: all banks once);  V image: [8 keys][channel] pieces.
-// The running maximum of a row moves only when a score passes it by 2^8 (fp32 sums and bf16 probabilities do not care about a common factor),
-// so the output is rarely rescaled.  Probabilities are rounded to bf16 once: their errors are independent and average out like the
-// values' own (measured 1.0-1.4 x the error of the rounded output), and a second product would cost 50 % of the matrix work.
+// The running reference of a row moves only when its probabilities outgrow 2^40 (fp32 sums and bf16 probabilities do not care about a common
+// factor), so the common step takes no maximum.  Probabilities are rounded to bf16 once, and the sums are of the rounded ones: their errors are
+// independent and average out like the values' own (measured 1.0-1.4 x the error of the rounded output); a second product for their low parts
+// would cost 50 % of the matrix work.
+// 4 sequences x 16 heads of 128, 1024 queries over 2976-4000 keys: 140 us (0.83 PFLOP/s; 156 with a maximum a tile).  The products and their
+// operand reads alone take 53 us, with the staging 62: what binds it are the vector instructions of the softmax (130 a tile and wave), which two
+// waves of a SIMD in the same phase do not hide behind each other's products.  Opposite phases for the two halves of the workgroup, a barrier
+// between the phases, took 151; softmax of one tile beside the products of another within a wave 155.
 template <int HD>
 __device__ __forceinline__ int kimg(int row, int piece) {
   constexpr int PC = HD / 8, SH = HD == 128 ? 0 : HD == 64 ? 1 : 2;
@@ -305,19 +315,22 @@ template <int HD, int DT, int NW>
 __global__ __launch_bounds__(NW * 64) void attn_kv8_tile_kernel(AttnArgs a) {
   constexpr int NC = HD / 32, NK = HD / 16;
   constexpr int IMG = KT * HD * 2;                        // bytes of one image
-  constexpr int UNITS = KT * HD / 16;                     // 16-byte pieces of K (and of V) in a tile
+  constexpr int UNITS = KT * HD / 16;                     // 16-byte pieces of K, and of V, in a tile
   constexpr int NT = NW * 64;
-  constexpr int UPT = (2 * UNITS + NT - 1) / NT;          // pieces per thread
-  __shared__ __attribute__((aligned(16))) char smem[2][2 * IMG];
+  constexpr int UPT = (UNITS + NT - 1) / NT;              // pieces per thread
+  constexpr int RT = NW * 32;
+  __shared__ __attribute__((aligned(16))) char kimgs[2][IMG];
+  __shared__ __attribute__((aligned(16))) char vimgs[2][IMG];
   const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
   const int r = lane & 31, hf = lane >> 5;
-  const int split = blockIdx.x % a.splits, rt = a.rtiles - 1 - blockIdx.x / a.splits;     // the row tiles with the most keys first
-  const int h = blockIdx.y, s = blockIdx.z;
-  constexpr int RT = NW * 32;
+  // consecutive row tiles of a head on one XCD (they read the same keys), those with the most keys first
+  const int id = xcd_remap(blockIdx.x, gridDim.x);
+  const int split = id % a.splits, rt = a.rtiles - 1 - id / a.splits % a.rtiles;
+  const int hs = id / (a.splits * a.rtiles), h = hs % a.H, s = hs / a.H;
   const Span sp = span_of(a, s, rt * RT, rt * RT + RT);
   if (sp.rows == 0) return;
   const int per = (sp.nt + a.splits - 1) / a.splits;
-  const int i0 = split * per, i_end = min(sp.nt, i0 + per);
+  const int i0 = split * per, n = min(sp.nt, i0 + per) - i0;      // this workgroup's tiles
   const long head = (long)s * a.H + h;
   const uint8_t* kb = a.k8 + head * a.cap * HD;
   const uint8_t* vb = a.v8 + head * a.cap * HD;
@@ -326,12 +339,9 @@ __global__ __launch_bounds__(NW * 64) void attn_kv8_tile_kernel(AttnArgs a) {
 
   const int row = rt * RT + wave * 32 + r;
   const int w0 = rt * RT + wave * 32;                     // the wave's first row
-  // two waves share a SIMD (i and i + 4): the first goes ahead, so that its exponentials run beside the other's products
-  if (NW == 8 && wave < 4) __builtin_amdgcn_s_setprio(1);
-  const bool wave_on = w0 < sp.rows;
-  const int rc = min(row, sp.rows - 1);
+  const int rc = min(row, sp.rows - 1);                   // (lanes and waves behind the last row compute it again and write nothing)
   const int t = rc / a.G, gq = rc - t * a.G;
-  const int prow = sp.p0 + t;
+  const Sight sight = sight_of(a, sp, sp.p0 + t);
   const int wfirst = sp.p0 + min(w0, sp.rows - 1) / a.G, wlast = sp.p0 + min(w0 + 31, sp.rows - 1) / a.G;
   bf16x8_v qf[NK];
   {
@@ -339,161 +349,208 @@ __global__ __launch_bounds__(NW * 64) void attn_kv8_tile_kernel(AttnArgs a) {
 #pragma unroll
     for (int k = 0; k < NK; ++k) qf[k] = *reinterpret_cast<const bf16x8_v*>(qp + k * 16);
   }
-  f32x16 o[NC];
+  f32x16 o[NC], sc[2];
 #pragma unroll
   for (int c = 0; c < NC; ++c)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[c][i] = 0.f;
   float m = NEVER, l = 0.f;
+  bf16x8_v pf[4];
   // the queries are waited for here: left to the first product, that wait would stand in the key loop and cover the prefetch there too
 #pragma unroll
   for (int k = 0; k < NK; ++k) asm volatile("" : "+v"(qf[k]));
 
-  uint4 st[UPT];
-  float ss[UPT];
-  auto fetch = [&](int tile) {
+  // ---- pieces of 16 bytes on their way in: UPT of a K tile, UPT of a V tile per thread ----
+  uint4 kst[UPT], vst[UPT];
+  float kss[UPT], vss[UPT];
+  uint32_t off[UPT];
+  int kblk[UPT], vblk[UPT];
 #pragma unroll
-    for (int i = 0; i < UPT; ++i) {
-      const int u = tid + i * NT;                         // [0, UNITS): K, then V
-      if (2 * UNITS % NT && u >= 2 * UNITS) break;
-      const bool v = u >= UNITS;
-      const int uu = v ? u - UNITS : u;
-      st[i] = *reinterpret_cast<const uint4*>((v ? vb : kb) + (long)tile * KT * HD + uu * 16);
-      const int key = v ? (uu / HD) * 16 : uu / (HD / 16);
-      ss[i] = (v ? vsb : ksb)[(tile * KT + key) >> a.bshift];
-    }
+  for (int i = 0; i < UPT; ++i) {
+    const int u = min(tid + i * NT, UNITS - 1);
+    off[i] = u * 16;
+    kblk[i] = (u / (HD / 16)) >> a.bshift;
+    vblk[i] = ((u / HD) * 16) >> a.bshift;
+  }
+  auto fetch_k = [&](int j) {
+    if (j >= n) return;
+    const int tile = tile_of(sp, i0 + j);
+    const uint8_t* base = kb + (long)tile * (KT * HD);
+    const float* sb = ksb + ((tile * KT) >> a.bshift);
+#pragma unroll
+    for (int i = 0; i < UPT; ++i) { kst[i] = *reinterpret_cast<const uint4*>(base + off[i]); kss[i] = sb[kblk[i]]; }
   };
-  auto stage = [&](int tile, char* img) {
-    const bool edge = tile * KT < sp.first || tile * KT + KT - 1 > sp.plast;      // positions out there hold whatever was left: zeros
+  auto fetch_v = [&](int j) {
+    if (j >= n) return;
+    const int tile = tile_of(sp, i0 + j);
+    const uint8_t* base = vb + (long)tile * (KT * HD);
+    const float* sb = vsb + ((tile * KT) >> a.bshift);
+#pragma unroll
+    for (int i = 0; i < UPT; ++i) { vst[i] = *reinterpret_cast<const uint4*>(base + off[i]); vss[i] = sb[vblk[i]]; }
+  };
+  auto put = [&](char* img, int at0, int at1, const uint32_t (&w)[4], float sc8) {
+    *reinterpret_cast<uint4*>(img + at0) = make_uint4(kv8_unpack2<DT, false>(w[0], sc8), kv8_unpack2<DT, true>(w[0], sc8),
+                                                      kv8_unpack2<DT, false>(w[1], sc8), kv8_unpack2<DT, true>(w[1], sc8));
+    *reinterpret_cast<uint4*>(img + at1) = make_uint4(kv8_unpack2<DT, false>(w[2], sc8), kv8_unpack2<DT, true>(w[2], sc8),
+                                                      kv8_unpack2<DT, false>(w[3], sc8), kv8_unpack2<DT, true>(w[3], sc8));
+  };
+  // positions outside [first, plast] hold whatever was left there: zeros
+  auto stage_k = [&](int j, char* img) {
+    if (j >= n) return;
+    const int tk = tile_of(sp, i0 + j) * KT;
+    const bool edge = tk < sp.first || tk + KT - 1 > sp.plast;
 #pragma unroll
     for (int i = 0; i < UPT; ++i) {
       const int u = tid + i * NT;
-      if (2 * UNITS % NT && u >= 2 * UNITS) break;
-      const bool v = u >= UNITS;
-      const int uu = v ? u - UNITS : u;
-      uint32_t w[4] = {st[i].x, st[i].y, st[i].z, st[i].w};
-      float sc = ss[i];
-      int at0, at1;
-      if (!v) {
-        const int key = uu / (HD / 16), cc = uu % (HD / 16);
-        const int kk = key & 31;                          // its row in the half tile
-        const int lr = (key & 32) + 8 * ((kk >> 2) & 3) + 4 * (kk >> 4) + (kk & 3);
-        at0 = kimg<HD>(lr, 2 * cc);
-        at1 = kimg<HD>(lr, 2 * cc + 1);
-        if (edge && (tile * KT + key < sp.first || tile * KT + key > sp.plast)) {
-          w[0] = w[1] = w[2] = w[3] = 0;
-          sc = 0.f;
-        }
-      } else {
-        const int t16 = uu / HD, ch = uu % HD;
-        at0 = IMG + ((2 * t16) * HD + ch) * 16;
-        at1 = at0 + HD * 16;
-        if (edge) {
-          const int lo = sp.first - (tile * KT + t16 * 16), hi = sp.plast - (tile * KT + t16 * 16);
-#pragma unroll
-          for (int d = 0; d < 4; ++d) {
-            uint32_t bm = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (4 * d + e >= lo && 4 * d + e <= hi) bm |= 0xffu << (8 * e);
-            w[d] &= bm;
-          }
-          if (lo > 15 || hi < 0) sc = 0.f;
-        }
+      if (UNITS % NT && u >= UNITS) break;
+      uint32_t w[4] = {kst[i].x, kst[i].y, kst[i].z, kst[i].w};
+      float sc8 = kss[i];
+      const int key = u / (HD / 16), cc = u % (HD / 16);
+      const int kk = key & 31;                            // its row in the half tile
+      const int lr = (key & 32) + 8 * ((kk >> 2) & 3) + 4 * (kk >> 4) + (kk & 3);
+      if (edge && (tk + key < sp.first || tk + key > sp.plast)) {
+        w[0] = w[1] = w[2] = w[3] = 0;
+        sc8 = 0.f;
       }
-      *reinterpret_cast<uint4*>(img + at0) = make_uint4(kv8_unpack2<DT, false>(w[0], sc), kv8_unpack2<DT, true>(w[0], sc), kv8_unpack2<DT, false>(w[1], sc),
-                                                        kv8_unpack2<DT, true>(w[1], sc));
-      *reinterpret_cast<uint4*>(img + at1) = make_uint4(kv8_unpack2<DT, false>(w[2], sc), kv8_unpack2<DT, true>(w[2], sc), kv8_unpack2<DT, false>(w[3], sc),
-                                                        kv8_unpack2<DT, true>(w[3], sc));
+      put(img, kimg<HD>(lr, 2 * cc), kimg<HD>(lr, 2 * cc + 1), w, sc8);
     }
   };
-  if (i0 < i_end) {
-    fetch(tile_of(sp, i0));
-    stage(tile_of(sp, i0), smem[0]);
-  }
-  __syncthreads();
-  for (int it = i0; it < i_end; ++it) {
-    const int tile = tile_of(sp, it);
-    const char* img = smem[(it - i0) & 1];
-    const bool more = it + 1 < i_end;
-    if (more) fetch(tile_of(sp, it + 1));
-    const int tk = tile * KT;
-    if (wave_on && tk <= wlast) {
-      const bool plain = tk >= sp.first && tk + KT - 1 <= wfirst && (a.window == 0 || tk > wlast - a.window);
-      f32x16 sc[2];
-      auto scores = [&]() {
+  auto stage_v = [&](int j, char* img) {
+    if (j >= n) return;
+    const int tk = tile_of(sp, i0 + j) * KT;
+    const bool edge = tk < sp.first || tk + KT - 1 > sp.plast;
 #pragma unroll
-        for (int k = 0; k < NK; ++k)
+    for (int i = 0; i < UPT; ++i) {
+      const int u = tid + i * NT;
+      if (UNITS % NT && u >= UNITS) break;
+      uint32_t w[4] = {vst[i].x, vst[i].y, vst[i].z, vst[i].w};
+      float sc8 = vss[i];
+      const int t16 = u / HD, ch = u % HD;
+      if (edge) {
+        const int lo = sp.first - (tk + t16 * 16), hi = sp.plast - (tk + t16 * 16);
 #pragma unroll
-          for (int kt = 0; kt < 2; ++kt) {
-            const bf16x8_v kf = *reinterpret_cast<const bf16x8_v*>(img + kimg<HD>(kt * 32 + r, 2 * k + hf));
-            sc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[k], sc[kt], 0, 0, 0);
-          }
-        // operand reads run AHEAD products before their use (scheduled next to it, every product waited for its own read)
-        constexpr int AHEAD = 2 * NK < 6 ? 2 * NK : 6;
-        __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+        for (int d = 0; d < 4; ++d) {
+          uint32_t bm = 0;
 #pragma unroll
-        for (int i = 0; i < 2 * NK - AHEAD; ++i) {
-          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          for (int e = 0; e < 4; ++e)
+            if (4 * d + e >= lo && 4 * d + e <= hi) bm |= 0xffu << (8 * e);
+          w[d] &= bm;
         }
-        __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
-      };
-      // the mask is what the products start from, 0 or -inf (positions outside [first, plast] were zeroed on their way into LDS): the scores are
-      // written by the products alone and stay where those leave them
-      if (plain) {
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) sc[kt][i] = 0.f;
-        scores();
-      } else {
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) sc[kt][i] = visible(a, sp, tk + kt * 32 + hf * 16 + i, prow) ? 0.f : -INFINITY;
-        scores();
+        if (lo > 15 || hi < 0) sc8 = 0.f;
       }
-      {
-        float mx = sc[0][0];
+      put(img, ((2 * t16) * HD + ch) * 16, ((2 * t16 + 1) * HD + ch) * 16, w, sc8);
+    }
+  };
+
+  // Scores of tile j.  The mask is what the products start from, 0 or -inf: the scores are written by the products alone, in place.
+  auto k_frag = [&](const char* img, int kt, int k) { return *reinterpret_cast<const bf16x8_v*>(img + kimg<HD>(kt * 32 + r, 2 * k + hf)); };
+  auto first_scores = [&](int j, const char* img) {
+    const int tk = tile_of(sp, i0 + j) * KT;
+    const bool plain = tk >= sp.first && tk + KT - 1 <= wfirst && (a.window == 0 || tk > wlast - a.window);
+    if (plain) {
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
+      for (int kt = 0; kt < 2; ++kt) {
+        f32x16 z;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[kt][i]);
-        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-        mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * a.scale_log2e;        // scale > 0 (checked on entry)
-        if (__builtin_amdgcn_ballot_w64(mx > m + 8.0f)) {
-          const float mn = fmaxf(m, mx);
-          const float alpha = __builtin_amdgcn_exp2f(m - mn);
-          m = mn;
-          l *= alpha;
+        for (int i = 0; i < 16; ++i) z[i] = 0.f;
+        sc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_frag(img, kt, 0), qf[0], z, 0, 0, 0);
+      }
+    } else {
 #pragma unroll
-          for (int c = 0; c < NC; ++c)
+      for (int kt = 0; kt < 2; ++kt) {
+        f32x16 z;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[c][i] *= alpha;
-        }
-        float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            float y[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = __builtin_amdgcn_exp2f(fmaf(sc[kt][8 * u + e], a.scale_log2e, -m));
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) { sum0 += y[e]; sum1 += y[e + 1]; }
-            const bf16x8_v pf = pack8_bf16(y);
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-              const bf16x8_v vf = *reinterpret_cast<const bf16x8_v*>(img + IMG + ((kt * 4 + 2 * hf + u) * HD + c * 32 + r) * 16);
-              o[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf, o[c], 0, 0, 0);
-            }
-          }
-        l += sum0 + sum1;
+        for (int i = 0; i < 16; ++i) z[i] = visible(sight, tk + kt * 32 + hf * 16 + i) ? 0.f : -INFINITY;
+        sc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_frag(img, kt, 0), qf[0], z, 0, 0, 0);
       }
     }
-    if (more) stage(tile_of(sp, it + 1), smem[(it + 1 - i0) & 1]);
+  };
+  auto more_scores = [&](const char* img) {
+#pragma unroll
+    for (int k = 1; k < NK; ++k)
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) sc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_frag(img, kt, k), qf[k], sc[kt], 0, 0, 0);
+  };
+  auto output = [&](const char* img) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const bf16x8_v vf = *reinterpret_cast<const bf16x8_v*>(img + (((q >> 1) * 4 + 2 * hf + (q & 1)) * HD + c * 32 + r) * 16);
+        o[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[q], o[c], 0, 0, 0);
+      }
+  };
+
+  // ---- probabilities against the running reference as it stands; a lane whose sum of 32 passes 2^40 (or is infinite: the first
+  // visible keys) sends the wave back for the maximum.  Sums are of the rounded probabilities, two an instruction. ----
+  auto softmax = [&]() {
+    float sum;
+    auto probabilities = [&]() {
+      float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = __builtin_amdgcn_exp2f(fmaf(sc[q >> 1][8 * (q & 1) + e], a.scale_log2e, -m));
+        pf[q] = pack8_bf16(y);
+        const uint4 w = __builtin_bit_cast(uint4, pf[q]);
+        const bf16x2_t one = {(__bf16)1.0f, (__bf16)1.0f};
+        s0 = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w.x), one, s0, false);
+        s1 = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w.y), one, s1, false);
+        s0 = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w.z), one, s0, false);
+        s1 = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w.w), one, s1, false);
+      }
+      sum = s0 + s1;
+    };
+    probabilities();
+    if (__builtin_amdgcn_ballot_w64(!(sum <= 0x1p40f))) {
+      float mx = sc[0][0];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[kt][i]);
+      const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+      mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * a.scale_log2e;        // scale > 0 (checked on entry)
+      const float mn = fmaxf(m, mx);
+      const float alpha = __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[c][i] *= alpha;
+      probabilities();
+    }
+    l += sum;
+  };
+
+  if (n > 0) {
+    fetch_k(0);
+    fetch_v(0);
+    stage_k(0, kimgs[0]);
+    stage_v(0, vimgs[0]);
+    fetch_k(1);
+    fetch_v(1);
     __syncthreads();
+    // step j, its parity known to the compiler: LDS addresses are registers + constants
+    auto step = [&](int j, auto parity) {
+      constexpr int p = parity;
+      first_scores(j, kimgs[p]);
+      more_scores(kimgs[p]);
+      softmax();
+      stage_k(j + 1, kimgs[p ^ 1]);                       // requested a whole step ago; its last readers are behind the barrier
+      stage_v(j + 1, vimgs[p ^ 1]);
+      fetch_k(j + 2);
+      fetch_v(j + 2);
+      output(vimgs[p]);
+      __syncthreads();
+    };
+    int j = 0;
+    for (; j + 1 < n; j += 2) {
+      step(j, std::integral_constant<int, 0>{});
+      step(j + 1, std::integral_constant<int, 1>{});
+    }
+    if (j < n) step(j, std::integral_constant<int, 0>{});
   }
   l += __shfl_xor(l, 32, 64);
   if (row >= sp.rows) return;
@@ -597,8 +654,9 @@ int keys_of(int cap, int T, int window, int sinks, int max_len) {
 template <int HD, int DT>
 int launch_rows(const AttnArgs& a, const Plan& p, hipStream_t s) {
   const dim3 grid((unsigned)(p.splits * p.rtiles), a.H, a.S);
-  if (p.tiled && p.nw == 4) hipLaunchKernelGGL((attn_kv8_tile_kernel<HD, DT, 4>), grid, dim3(256), 0, s, a);
-  else if (p.tiled) hipLaunchKernelGGL((attn_kv8_tile_kernel<HD, DT, 8>), grid, dim3(512), 0, s, a);
+  const dim3 flat((unsigned)(p.splits * p.rtiles) * a.H * a.S);
+  if (p.tiled && p.nw == 4) hipLaunchKernelGGL((attn_kv8_tile_kernel<HD, DT, 4>), flat, dim3(256), 0, s, a);
+  else if (p.tiled) hipLaunchKernelGGL((attn_kv8_tile_kernel<HD, DT, 8>), flat, dim3(512), 0, s, a);
   else if (p.nq == 1) hipLaunchKernelGGL((attn_kv8_rows_kernel<HD, DT, 1, 8>), grid, dim3(512), 0, s, a);
   else if (p.nq == 2) hipLaunchKernelGGL((attn_kv8_rows_kernel<HD, DT, 2, 4>), grid, dim3(256), 0, s, a);
   else if constexpr (HD < 128) hipLaunchKernelGGL((attn_kv8_rows_kernel<HD, DT, 4, 4>), grid, dim3(256), 0, s, a);
@@ -630,6 +688,7 @@ int neko_attn_kv8_impl(const uint8_t* k8, const uint8_t* v8, const float* ks, co
   const Plan p = plan_of(S, H, hd, T * G, keys_of(cap, T, window, sinks, max_len));
   const long need = p.splits > 1 ? (long)S * H * p.splits * p.rtiles * p.rt * (hd + 2) : 0;
   if (need > ws_floats || (need && !ws)) return NEKO_ERR_ARG;
+  if ((long)S * H * p.splits * p.rtiles > 0x7fffffffL) return NEKO_ERR_UNSUPPORTED;
   const int bshift = block == 16 ? 4 : block == 32 ? 5 : 6;
   AttnArgs a{k8, v8, ks, vs, q, out, q_ss, q_st, o_ss, o_st, pos, n_new, start, ws, nullptr, S, H, G, cap, T, bshift, window, sinks, p.splits, p.rtiles,
              scale * 1.4426950408889634f};
