@@ -66,15 +66,16 @@ __device__ __forceinline__ double pow2_64(double x) {
   const double r = pow2_64_above_1000(x);
   return x > -1000.0 ? r : 0.0;
 }
-// weight of logit l under the maximum m, c = log2(e) / tau: 2^(c l - c m); an infinite maximum shares the mass among its equals
+// weight of logit l under the maximum m, c = log2(e) / tau: 2^((l - m) c), exactly 1 for the maximum at any temperature (c l - c m in one multiply-add
+// is off by the rounding of c m); an infinite maximum shares the mass among its equals
 struct Weigh {
-  double c, cm;
+  double c;
   float m;
   bool inf;
-  __device__ __forceinline__ Weigh(float m_, double c_) : c(c_), cm((double)m_ * c_), m(m_), inf(m_ == INFINITY || m_ == -INFINITY) {}
+  __device__ __forceinline__ Weigh(float m_, double c_) : c(c_), m(m_), inf(m_ == INFINITY || m_ == -INFINITY) {}
   __device__ __forceinline__ double operator()(float l) const {
     if (__builtin_expect(inf, 0)) return l == m && m == INFINITY ? 1.0 : 0.0;
-    return pow2_64(fma((double)l, c, -cm));
+    return pow2_64(((double)l - (double)m) * c);
   }
 };
 __device__ __forceinline__ double wave_sum64(double v) {
@@ -93,7 +94,7 @@ __device__ __forceinline__ double wave_scan64(double v, int lane) {       // inc
 __device__ __forceinline__ int drafted(const VerifyArgs& a, int b) { return min(max(a.n_draft ? a.n_draft[b] : a.K, 0), a.K); }
 
 // ---- launch 1: every row piece -> maximum and sum (or the maximum's index) ----
-// Bound by the vector unit: an element costs 20 instructions (15 of them fp64), so everything else stays out of the loop: whole pieces load and
+// Bound by the vector unit: an element costs 21 instructions (16 of them fp64), so everything else stays out of the loop: whole pieces load and
 // compare without bounds, and a NaN needs no test (the maximum ignores it, the lower bound of the exponent turns it into nothing).
 template <typename T, bool GREEDY>
 __global__ __launch_bounds__(VT) void verify_rows_kernel(VerifyArgs a) {
@@ -150,10 +151,10 @@ __global__ __launch_bounds__(VT) void verify_rows_kernel(VerifyArgs a) {
 #pragma unroll
     for (int e = 0; e < VE; ++e) s += x[e] == bm && bm == INFINITY ? 1.0 : 0.0;
   } else {
-    const double cm = (double)bm * a.c;
+    const double dm = (double)bm;
     // exponents stop at -1000: 2^-1000 beside the 1 of the maximum is nothing, and the exponent field does not run over
 #pragma unroll
-    for (int e = 0; e < VE; ++e) s += pow2_64_above_1000(fmax(fma((double)x[e], a.c, -cm), -1000.0));
+    for (int e = 0; e < VE; ++e) s += pow2_64_above_1000(fmax(((double)x[e] - dm) * a.c, -1000.0));
   }
   s = wave_sum64(s);
   if (lane == 0) ss[wave] = s;
@@ -409,7 +410,7 @@ int launch(const VerifyArgs& a, hipStream_t s) {
 
 long neko_verify_draft_ws_bytes_impl(int B, int K, int V) {
   if (B <= 0 || K <= 0 || V <= 0) return 0;
-  const long pieces = (V + PIECE - 1) / PIECE;
+  const long pieces = ((long)V + PIECE - 1) / PIECE;
   return (long)B * pieces * ((2 * K + 1) * 12L + 16L) + (long)B * (long)sizeof(Source);
 }
 
@@ -418,12 +419,12 @@ int neko_verify_draft_impl(const void* target, long t_sb, long t_sr, const void*
                            long long* out, void* ws, long ws_bytes, hipStream_t s) {
   if (!target || !tokens || !accepted || !out || !ws || B <= 0 || K <= 0 || V <= 0) return NEKO_ERR_ARG;
   if (!(temperature >= 0.f) || (temperature > 0.f && (!u || !r))) return NEKO_ERR_ARG;
-  if (K > MAXK - 1 || B > 65535) return NEKO_ERR_UNSUPPORTED;
+  if (K > MAXK - 1 || B > 65535 || V > (1 << 30)) return NEKO_ERR_UNSUPPORTED;
   if ((uintptr_t)ws & 7 || ws_bytes < neko_verify_draft_ws_bytes_impl(B, K, V)) return NEKO_ERR_ARG;
   VerifyArgs a{};
   a.target = target; a.draft = draft; a.t_sb = t_sb; a.t_sr = t_sr; a.d_sb = d_sb; a.d_sr = d_sr;
   a.tokens = tokens; a.u = u; a.r = r; a.n_draft = n_draft; a.accepted = accepted; a.out = out;
-  a.B = B; a.K = K; a.V = V; a.pieces = (V + PIECE - 1) / PIECE;
+  a.B = B; a.K = K; a.V = V; a.pieces = (int)(((long)V + PIECE - 1) / PIECE);
   const long cells = (long)B * (2 * K + 1) * a.pieces;
   a.ps = (double*)ws;
   a.pw = a.ps + cells;

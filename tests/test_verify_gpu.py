@@ -118,3 +118,13 @@ def test_verify_keeps_the_target_distribution():
     freq = torch.bincount(out[:, 0].cpu(), minlength=V).double() / N
     p = torch.softmax(t.double(), 0)
     assert bool(((freq - p).abs() <= 4 * (p * (1 - p) / N).sqrt()).all()), (freq, p)
+
+
+@pytest.mark.parametrize("temperature", [1e-3, 1e-12, 1e-30])
+@pytest.mark.parametrize("with_draft", [True, False])
+def test_verify_cold(temperature, with_draft):
+    """Temperatures next to zero: the largest logit has all the mass, in every piece of the row, whatever logit / temperature comes to."""
+    t, x, d, u, r, n = _case(6, 4, 9001, 1.0, with_draft, torch.float32, seed=8)
+    x[:4] = t[:4, :4].argmax(-1)
+    c = (t, x, d, u, r, n)
+    assert _run(*c, temperature) == verify(*c, temperature)
