@@ -373,6 +373,8 @@ int neko_patch_pos_add_bwd_sorted(const float* dout, const int* hkeys_sorted, co
  * neko_attn_kv8: T rows a sequence at positions pos[s] + i (i < n as above; other rows of `out` are left as they are), G query heads per key
  *   head (query head h * G + g reads key head h), q and out bf16 with strides as k above.  Row at position p sees t with start[s] <= t <= p and,
  *   where window > 0, t > p - window or t < start[s] + sinks (start NULL: 0).  A row that sees nothing is 0.  `scale` > 0 multiplies q . k.
+ *   `out` may be q itself, rows beside q's in one buffer or memory of its own; rows that overlap otherwise are refused.  Scores are held for
+ *   |scale q . k| up to 2^29.
  *   What lies in the cache outside [start, last row] never reaches the output.  max_len: host-known bound on pos + T (0: cap); it sizes
  *   the split of the key axis and changes no result beyond rounding.  ws: neko_attn_kv8_ws_floats(..) floats (may be 0), private to the call.
  * neko_verify_draft: sequence b, K + 1 rows of target logits (element (b, i, v) at b * t_sb + i * t_sr + v; fp32 or bf16), n = n_draft[b] <= K
@@ -381,12 +383,13 @@ int neko_patch_pos_add_bwd_sorted(const float* dout, const int* hkeys_sorted, co
  *   smallest v whose cumulative weight exceeds r times the total, weights max(p - q, 0) of the first row not kept (p where nothing is left),
  *   or p of row n.  temperature 0: kept while x_i is the row's largest logit (lowest index among equals), then the row's largest.
  *   out_tokens [B][K + 1]: the kept tokens, the next one, then -1.  NaN logits count as -inf; a row without a logit above -inf keeps
- *   nothing and gives the token -1.  K <= 62.
+ *   nothing and gives the token -1.  K <= 62, V <= 2^30.
  * neko_distill_topk: rows of R student logits z (fp32 or bf16, leading dimension ldz, columns >= V ignored) against k teacher logits and their
  *   indices (t_val, t_idx [R][k]; an index outside [0, V) is no entry; equal indices add up):
  *     loss_row = (1 - hard) tau^2 KL(softmax(t / tau) || softmax(z / tau)) + hard CE(z, target)      (target int64 [R], < 0: no such term)
  *     dlogits  = weight[r] d loss_row / dz in z's type, 0 in columns V .. Vpad-1; may be z itself; NULL: loss only
- *   weight 0: loss 0, gradient 0.  k <= 1024; Vpad, ldz, ldd multiples of 16 bytes. */
+ *   weight 0: loss 0, gradient 0.  k <= 1024; Vpad, ldz, ldd multiples of 16 bytes; tau at least the smallest normal number.  Rows of dlogits that
+ *   overlap z in part are refused. */
 int neko_kv8_append(void* k8, void* v8, float* k_scale, float* v_scale, int dtype, int nseq, int H, int cap, int hd, int block, const uint16_t* k,
                     long k_ss, long k_st, const uint16_t* v, long v_ss, long v_st, const int* pos, const int* n_new, int T, void* stream);
 int neko_kv8_read(const void* k8, const void* v8, const float* k_scale, const float* v_scale, int dtype, int nseq, int H, int cap, int hd,

@@ -685,6 +685,14 @@ int neko_attn_kv8_impl(const uint8_t* k8, const uint8_t* v8, const float* ks, co
   if (rc) return rc;
   if (T > cap || (long)T * G > (1 << 24)) return NEKO_ERR_ARG;
   if (((uintptr_t)q | (uintptr_t)out) & 15 || (q_ss | q_st | o_ss | o_st) & 7) return NEKO_ERR_ARG;
+  {
+    // rows and sequences in the order of their strides; every output row is written by its own workgroup, in no order
+    const bool in_rows = S == 1 || (T > 1 && o_st <= o_ss);
+    const long w = (long)H * G * hd * 2, n_lo = in_rows ? T : S, n_hi = in_rows ? S : T;
+    const long q_lo = 2 * (in_rows ? q_st : q_ss), q_hi = 2 * (in_rows ? q_ss : q_st), o_lo = 2 * (in_rows ? o_st : o_ss), o_hi = 2 * (in_rows ? o_ss : o_st);
+    if ((q_ss | q_st | o_ss | o_st) < 0 || !neko_rows_apart(w, n_lo, o_lo, n_hi, o_hi) || neko_rows_shared(q, q_lo, q_hi, out, o_lo, o_hi, w, n_lo, n_hi))
+      return NEKO_ERR_ARG;
+  }
   const Plan p = plan_of(S, H, hd, T * G, keys_of(cap, T, window, sinks, max_len));
   const long need = p.splits > 1 ? (long)S * H * p.splits * p.rtiles * p.rt * (hd + 2) : 0;
   if (need > ws_floats || (need && !ws)) return NEKO_ERR_ARG;

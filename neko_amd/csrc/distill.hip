@@ -94,8 +94,8 @@ template <> struct Piece<float> {
 // NCH > 0: the row lives in NCH pieces per thread, as it came (unpacked again in every pass: an unpacked bf16 row would be twice the registers
 // and half the workgroups per CU); 0: it is read again for every use.
 // TWO: labels at temperature 1 beside a teacher at another, two exponentials per element and pass.  The factor of a gradient term is folded into
-// its exponent (2^(c x + b), b = log2 of the factor - c m; -inf for a term that the row does not have): per element 0.5-1 issue slots for the
-// maximum, 7 (13 with TWO) for the sums, 7.5 (12.5) for the gradient, an exponential counting four.
+// its exponent (2^(c (x - m) + log2 of the factor); -inf for a term that the row does not have): per element 0.5-1 issue slots for the
+// maximum, 8 (14 with TWO) for the sums, 8.5 (13.5) for the gradient, an exponential counting four.
 // two workgroups of 1024 per CU where the row leaves room (64 registers): one loads while the other computes
 template <typename T, int NT, int NCH, bool TWO>
 __global__ __launch_bounds__(NT, NCH <= 7 ? 8 : NT == 512 ? 6 : 4) void distill_kernel(DistillArgs a) {
@@ -229,8 +229,8 @@ __global__ __launch_bounds__(NT, NCH <= 7 ? 8 : NT == 512 ? 6 : 4) void distill_
   // sums: c1 serves the teacher's temperature (and the labels where that is 1 or there is no teacher), LOG2E the labels' with TWO
   const bool soft = soft_w != 0.f && s_teacher[1] != 0.f;
   const float c1 = soft_w != 0.f ? LOG2E / a.tau : LOG2E;
-  // 2^(c x - n), n = c m rounded to an integer: the fused multiply-add then rounds once, relative to the exponent itself
-  const float b1 = -rintf(m * c1), b2 = -rintf(m * LOG2E);
+  // exponents are (x - m) c: exactly 0 for the maximum, whatever its size (c x - c m in one multiply-add is off by the rounding of c m, which a row
+  // of the type's lowest values or a tiny tau makes larger than any exponent fp32 can hold)
   float s1 = 0.f, s2 = 0.f;
   keep_packed();
 #pragma unroll
@@ -240,8 +240,9 @@ __global__ __launch_bounds__(NT, NCH <= 7 ? 8 : NT == 512 ? 6 : 4) void distill_
     else P::get(fence_cols(i, load(i)), x);
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      s1 += __builtin_amdgcn_exp2f(fmaf(x[e], c1, b1));
-      if (TWO) s2 += __builtin_amdgcn_exp2f(fmaf(x[e], LOG2E, b2));
+      const float d = x[e] - m;
+      s1 += __builtin_amdgcn_exp2f(d * c1);
+      if (TWO) s2 += __builtin_amdgcn_exp2f(d * LOG2E);
     }
   }
   s1 = wave_sum(s1);
@@ -260,13 +261,13 @@ __global__ __launch_bounds__(NT, NCH <= 7 ? 8 : NT == 512 ? 6 : 4) void distill_
 #pragma unroll 1
       for (int j = lane; j < a.k; j += 64) {
         const float t = __int_as_float(s_e[j].y);
-        if (t > 0.f) acc += t * fmaf(s_z[j], c1, b1);
+        if (t > 0.f) acc += t * ((s_z[j] - m) * c1);
       }
     acc = wave_sum(acc);
     if (lane == 0) {
       float loss = 0.f;
       if (soft) loss += soft_w * a.tau * a.tau * (s_teacher[0] + LN2 * (log2f(sum_soft) - acc));
-      if (has_y) loss += a.hard * LN2 * (log2f(sum_hard) - (TWO ? fmaf(zy, LOG2E, b2) : fmaf(zy, c1, b1)));
+      if (has_y) loss += a.hard * LN2 * (log2f(sum_hard) - (zy - m) * (TWO ? LOG2E : c1));
       a.loss_row[row] = loss;
     }
   }
@@ -276,7 +277,7 @@ __global__ __launch_bounds__(NT, NCH <= 7 ? 8 : NT == 512 ? 6 : 4) void distill_
   // is held to 2^-19 only)
   constexpr bool FOLD = sizeof(T) == 2;
   const float f1 = w * (TWO ? fs : fs + fh), f2 = w * fh;
-  const float e1 = FOLD ? b1 + __log2f(fabsf(f1)) : b1, e2 = FOLD ? b2 + __log2f(fabsf(f2)) : b2;
+  const float e1 = __log2f(fabsf(f1)), e2 = __log2f(fabsf(f2));
   const bool neg = FOLD && w < 0.f;
 #pragma unroll
   for (int i = 0; i < rounds; ++i) {
@@ -286,10 +287,11 @@ __global__ __launch_bounds__(NT, NCH <= 7 ? 8 : NT == 512 ? 6 : 4) void distill_
     else P::get(fence_cols(i, load(i)), x);
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      float g = __builtin_amdgcn_exp2f(fmaf(x[e], c1, e1));
+      const float d = x[e] - m;
+      float g = __builtin_amdgcn_exp2f(FOLD ? fmaf(d, c1, e1) : d * c1);
       if (!FOLD) g *= f1;
       if (TWO) {
-        const float g2 = __builtin_amdgcn_exp2f(fmaf(x[e], LOG2E, e2));
+        const float g2 = __builtin_amdgcn_exp2f(FOLD ? fmaf(d, LOG2E, e2) : d * LOG2E);
         g = FOLD ? g + g2 : fmaf(g2, f2, g);
       }
       x[e] = g;
@@ -313,9 +315,9 @@ __global__ __launch_bounds__(NT, NCH <= 7 ? 8 : NT == 512 ? 6 : 4) void distill_
         const int2 e = s_e[i];
         t += e.x == c ? __int_as_float(e.y) : 0.f;
       }
-      g += w * (fs * __builtin_amdgcn_exp2f(fmaf(x, c1, b1)) - soft_w * a.tau * t);
+      g += w * (fs * __builtin_amdgcn_exp2f((x - m) * c1) - soft_w * a.tau * t);
     }
-    if (has_y) g += w * (fh * __builtin_amdgcn_exp2f(TWO ? fmaf(x, LOG2E, b2) : fmaf(x, c1, b1)) - (c == (int)y ? a.hard : 0.f));
+    if (has_y) g += w * (fh * __builtin_amdgcn_exp2f((x - m) * (TWO ? LOG2E : c1)) - (c == (int)y ? a.hard : 0.f));
     return P::store(g);
   };
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // the dense values are written: a store behind the barrier to the same place comes second
@@ -353,11 +355,13 @@ int launch(const DistillArgs& a, int R, hipStream_t s) {
 int neko_distill_topk_impl(const void* z, long ldz, int is_bf16, int R, int V, int Vpad, const float* t_val, const int* t_idx, int k, const float* weight,
                            float tau, const long long* target, float hard, float* loss_row, void* dlogits, long ldd, hipStream_t s) {
   if (!z || !weight || R <= 0 || V <= 0 || Vpad < V || (!loss_row && !dlogits)) return NEKO_ERR_ARG;
-  if (!(tau > 0.f) || !(hard >= 0.f && hard <= 1.f) || (hard > 0.f && !target) || (hard < 1.f && (!t_val || !t_idx || k <= 0))) return NEKO_ERR_ARG;
+  if (!(tau >= 1.17549435e-38f) || !(hard >= 0.f && hard <= 1.f) || (hard > 0.f && !target) || (hard < 1.f && (!t_val || !t_idx || k <= 0))) return NEKO_ERR_ARG;
   if (k > KMAX) return NEKO_ERR_UNSUPPORTED;
   const int n = is_bf16 ? 8 : 4;
   if (Vpad % n || ldz % n || ldz < Vpad || (uintptr_t)z & 15) return NEKO_ERR_ARG;
   if (dlogits && (ldd % n || ldd < Vpad || (uintptr_t)dlogits & 15)) return NEKO_ERR_ARG;
+  const long width = (long)Vpad * (is_bf16 ? 2 : 4), size = is_bf16 ? 2 : 4;
+  if (dlogits && neko_rows_shared(z, ldz * size, 0, dlogits, ldd * size, 0, width, R, 1)) return NEKO_ERR_ARG;
   DistillArgs a{z, dlogits, ldz, ldd, V, Vpad, k, t_val, t_idx, weight, target, loss_row, tau, hard};
   return is_bf16 ? launch<bf16_t>(a, R, s) : launch<float>(a, R, s);
 }

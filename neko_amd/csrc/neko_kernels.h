@@ -171,3 +171,19 @@ int neko_verify_draft_impl(const void* target, long t_sb, long t_sr, const void*
                            long long* out, void* ws, long ws_bytes, hipStream_t s);
 int neko_distill_topk_impl(const void* z, long ldz, int is_bf16, int R, int V, int Vpad, const float* t_val, const int* t_idx, int k, const float* weight,
                            float tau, const long long* target, float hard, float* loss_row, void* dlogits, long ldd, hipStream_t s);
+
+// Rows of `w` bytes, lo bytes apart inside groups of n_lo, groups hi bytes apart (host side, for argument checks).  rows_apart: no two of them
+// overlap.  rows_shared: an output laid out like this at `out` would be written over input rows that others still read: anything but the same
+// rows, rows beside the input's in its own slots, or memory away from it.
+static inline bool neko_rows_apart(long w, long n_lo, long lo, long n_hi, long hi) {
+  return (n_lo == 1 || lo >= w) && (n_hi == 1 || hi >= (n_lo == 1 ? w : (n_lo - 1) * lo + w));
+}
+static inline bool neko_rows_shared(const void* in, long i_lo, long i_hi, const void* out, long o_lo, long o_hi, long w, long n_lo, long n_hi) {
+  const uintptr_t a = (uintptr_t)in, b = (uintptr_t)out;
+  const bool alike = (n_lo == 1 || i_lo == o_lo) && (n_hi == 1 || i_hi == o_hi);
+  if (a == b && alike) return false;
+  if (a + (uintptr_t)((n_lo - 1) * i_lo + (n_hi - 1) * i_hi + w) <= b || b + (uintptr_t)((n_lo - 1) * o_lo + (n_hi - 1) * o_hi + w) <= a) return false;
+  const uintptr_t d = a < b ? b - a : a - b;
+  const uintptr_t slot = (uintptr_t)(n_lo > 1 ? o_lo : n_hi > 1 ? o_hi : 0);
+  return !(alike && d >= (uintptr_t)w && d + (uintptr_t)w <= slot && (n_lo == 1 || n_hi == 1 || o_hi >= n_lo * o_lo));
+}

@@ -134,3 +134,48 @@ def test_distill_captured_and_loss_only():
         ops.distill_topk(z, V, Vpad, tv, ti, w, tau=2.0, loss_row=l2, dlogits=d2)
         ops.distill_topk(z, V, Vpad, tv, ti, w, tau=2.0, loss_row=l3)
         assert torch.equal(loss, l2) and torch.equal(dz, d2) and torch.equal(l2, l3)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [300, 30000, 120001])
+def test_distill_lowest_values(V, dtype):
+    """Logits of the type's lowest value: a row that holds nothing else is a flat one, and beside ordinary logits they count as -inf."""
+    z, Vpad, tv, ti, w, y = _case(3, V, 6, dtype, seed=V)
+    low = torch.finfo(dtype).min
+    flat = z.clone()
+    flat[:, :V] = low
+    for tau, hard in ((1.0, 0.0), (2.0, 0.4), (0.5, 1.0)):
+        _check(flat, V, Vpad, tv, ti, w, y, tau, hard)
+    ti = ti % 50
+    y = y % 50
+    a, b = z.clone(), z.clone()
+    a[:, 50:V], b[:, 50:V] = low, -math.inf
+    for tau, hard in ((1.0, 0.0), (2.0, 0.4), (0.5, 1.0)):
+        got, want = _run(a, V, Vpad, tv, ti, w, y, tau, hard), _run(b, V, Vpad, tv, ti, w, y, tau, hard)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        assert bool(torch.isfinite(got[0]).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("tau", [1e-6, 1e-12])
+def test_distill_cold(tau, dtype):
+    """tau next to zero: both distributions are one token, the loss is tau times the gap between them."""
+    R, V, k = 3, 2000, 4
+    z, Vpad, tv, ti, w, y = _case(R, V, k, dtype, seed=2)
+    best = torch.tensor([5, 900, 1999])
+    z[torch.arange(R), best] = 20.0
+    tv[:, 1] = 50.0
+    loss, dz = _run(z, V, Vpad, tv, ti, w, y, tau, 0.0)
+    for r in range(R):
+        t, s = int(ti[r, 1]), int(best[r])
+        gap = tau * (20.0 - float(z[r, t]))
+        # half a step of fp32 each: tau, log2(e), their quotient, the difference, its product with it, ln 2, the product with that, (1 - hard) tau tau
+        # in two products, and the last one
+        assert abs(float(loss[r]) - gap) <= 10 * 2.0 ** -24 * gap
+        want = torch.zeros(V, dtype=torch.float64)
+        want[s] += float(w[r]) * tau
+        want[t] -= float(w[r]) * tau
+        # bf16: the stored rounding, and the factor's logarithm (below 64 in size: half a step is 2^-19; a second one for the logarithm itself)
+        # in the exponent; fp32: four products
+        rel = 2.0 ** -8 + 2.0 ** -18 if dtype == torch.bfloat16 else 4 * 2.0 ** -24 + 2.0 ** -22
+        assert bool(((dz[r, :V].double() - want).abs() <= rel * want.abs()).all())

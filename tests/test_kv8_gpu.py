@@ -270,3 +270,54 @@ def test_two_streams_and_capture():
         other = eager(I8)
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(other, want[I8])
+
+
+@pytest.mark.parametrize("hd", [32, 128])
+@pytest.mark.parametrize("T", [1, 20, 150])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_attn_rising_and_falling_scores(hd, T, sign):
+    """Scores that climb (or fall) by some hundreds along the keys: the running reference moves many times, or never after the first keys."""
+    from neko_amd import ops
+    S, H, cap = 1, 2, 512
+    g = torch.Generator().manual_seed(T + hd)
+    u = torch.randn(1, 1, H, hd, generator=g)
+    ramp = sign * torch.linspace(-60.0, 60.0, cap).view(1, cap, 1, 1)
+    k = (ramp * u / hd ** 0.5 + 0.1 * torch.randn(S, cap, H, hd, generator=g)).to(BF16)
+    v = torch.randn(S, cap, H, hd, generator=g).to(BF16)
+    q = (8.0 * u + 0.1 * torch.randn(S, T, H, hd, generator=g)).to(BF16)
+    cache = ops.KV8Cache(S, H, cap, hd, dtype=E4, block=16)
+    ops.kv8_append(cache, k.cuda(), v.cuda(), _dev_i([0]))
+    pos = [cap - T]
+    got = ops.attn_kv8(cache, q.cuda(), _dev_i(pos))
+    kk, vv = (t.cpu().double().transpose(1, 2) for t in ops.kv8_read(cache, _dev_i([cap]), cap))
+    want, absv, big = attention(q, kk, vv, pos, [T], [0], 0, 0, hd ** -0.5, torch.zeros(S, T, H, hd))
+    # as in _attn_case, and the exponent (score and reference up to `big` in size): its fp32 roundings, four of big 2^-23 at most
+    p_round = 2.0 ** -8 if T > 64 else 2.0 ** -16
+    tol = 2.0 ** -8 * want.abs() + (p_round + (2 * hd + 8) * 2.0 ** -23 * big + cap * 2.0 ** -23 + 2.0 ** -21) * absv
+    err = (got.cpu().double() - want).abs()
+    assert bool((err <= tol).all()), float((err - tol).max())
+
+
+@pytest.mark.parametrize("window,sinks", [(90, 0), (200, 70), (1000, 3)])
+def test_attn_window_over_row_tiles(window, sinks):
+    """More rows than one row tile takes, with a window and sinks: tiles of keys that some of the rows see, in ragged sequences."""
+    _attn_case(3, 1, 2, 64, 1024, 300, [0, 500, 900], [300, 211, 300], [0, 130, 450], window, sinks, E4, 32, seed=window)
+
+
+@pytest.mark.parametrize("T", [1, 9, 150])
+def test_attn_in_place_and_beside(T):
+    """`out` may be q itself, or the rows beside q's in one buffer (query rows interleaved over sequences among them)."""
+    from neko_amd import ops
+    S, H, hd, cap = 3, 2, 64, 256
+    g = torch.Generator().manual_seed(T)
+    x = _rows(S, T, H, hd, g).cuda()
+    cache = ops.KV8Cache(S, H, cap, hd, dtype=I8, block=64)
+    pos = _dev_i([0, 40, 100])
+    ops.kv8_append(cache, x[:, :, 1], x[:, :, 2], pos)
+    want = ops.attn_kv8(cache, x[:, :, 0], pos)
+    turned = x.transpose(0, 1).contiguous().transpose(0, 1)              # rows of a position side by side
+    assert torch.equal(ops.attn_kv8(cache, turned[:, :, 0], pos, out=turned[:, :, 2]), want)
+    assert torch.equal(ops.attn_kv8(cache, x[:, :, 0], pos, out=x[:, :, 0]), want)
+    flat = want.clone()
+    with pytest.raises(RuntimeError):                                    # one output row for all sequences
+        ops.attn_kv8(cache, x[:, :, 1], pos, out=flat[:1].expand(S, T, H, hd))

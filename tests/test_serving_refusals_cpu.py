@@ -108,3 +108,21 @@ def test_plain_argument_errors():
                  lambda: ops.verify_draft(torch.zeros(1, 2, 9), torch.zeros(1, 1, dtype=torch.int64), temperature=-1.0)):
         with pytest.raises(AssertionError):
             call()
+
+
+@pytest.mark.parametrize("bad", [dict(q=P, out=P + 64, o_ss=64), dict(q=P, out=P + 64 * 1024, o_ss=32), dict(out=P + 64 * 1024, o_ss=0), dict(out=P + 128, o_ss=64),
+                                 dict(T=2, q_ss=128, o_ss=128, out=P + 16), dict(T=2, q_ss=128, o_ss=64, o_st=64, out=P + (1 << 20)), dict(q_ss=-64), dict(o_ss=-64),
+                                 dict(T=2, q_ss=256, q_st=128, o_ss=256, o_st=128, out=P + 64)], ids=str)
+def test_attn_refuses_shared_rows(bad):
+    """Output rows over one another or over rows of q that others still read."""
+    assert _rc("neko_attn_kv8", {**ATTN, "out": P + (1 << 20), **bad}.values()) == -1
+
+
+@pytest.mark.parametrize("bad", [dict(dl=P + 32), dict(dl=P + 16), dict(ldz=32, ldd=32, dl=P + 16), dict(ldz=32, ldd=32, dl=P + 48), dict(ldz=32), dict(tau=1e-39)], ids=str)
+def test_distill_refuses_shared_rows(bad):
+    assert _rc("neko_distill_topk", {**DISTILL, "R": 4, **bad}.values()) == -1
+
+
+def test_verify_refuses_long_rows():
+    assert _rc("neko_verify_draft", {**VERIFY, "V": (1 << 30) + 1, "ws_bytes": 1 << 40}.values()) == -2
+    assert _lib.load().neko_verify_draft_ws_bytes(1, 1, 2 ** 31 - 1) > 0
