@@ -749,7 +749,7 @@ def attn_kv8(cache: KV8Cache, q: torch.Tensor, pos: torch.Tensor, n_new: Optiona
     assert window >= 0 and sinks >= 0 and (sinks == 0 or window > 0), "sinks need a window"
     assert scale is None or scale > 0.0, "scale must be positive"
     if out is None:
-        out = (torch.empty if n_new is None and start is None else torch.zeros)((S, T, HG, hd), dtype=BF16, device=cache.device)
+        out = torch.zeros((S, T, HG, hd), dtype=BF16, device=cache.device)          # (positions outside the cache are no rows of the call either)
     To, o_ss, o_st, op = cache.row_strides(out, HG, "out", dev)
     assert To == T, "out must have q's rows"
     G = HG // H

@@ -866,6 +866,8 @@ class GatoPolicy(nn.Module):
             raise ValueError("the drafting policy must have the same vocabulary")
         if not deterministic and not temperature > 0:
             raise ValueError("temperature must be positive")
+        if max_length < 1:
+            raise ValueError("max_length must be positive")
         lo, hi = self.token_starts["text"], self.token_ends["text"]
         models = (self, draft)
         embs = [m.tokenize_input_dicts([batch_dict])[0][0].to(torch.float32) for m in models]
@@ -910,6 +912,8 @@ class GatoPolicy(nn.Module):
                 r = torch.rand(1, device=dev, generator=generator)
                 acc, out = ops.verify_draft(lt.unsqueeze(0), x.reshape(1, -1), draft_logits=torch.cat(dl).unsqueeze(0), u=u, r=r, temperature=temperature)
             new = [t for t in out[0].tolist() if t >= 0]         # the kept drafts and the token behind them (the step's one host read)
+            if not new:
+                raise RuntimeError("the policy's logits hold no number: no token to go on with")
             kept = len(new) - 1
             logits += [lt[i] for i in range(len(new))]
             tgt.truncate(base_t + 1 + kept)                  # the judged row and the kept drafts

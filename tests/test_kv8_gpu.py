@@ -321,3 +321,17 @@ def test_attn_in_place_and_beside(T):
     flat = want.clone()
     with pytest.raises(RuntimeError):                                    # one output row for all sequences
         ops.attn_kv8(cache, x[:, :, 1], pos, out=flat[:1].expand(S, T, H, hd))
+
+
+def test_attn_fresh_output_is_defined():
+    """Rows at positions outside the cache are no rows of the call: zeros in a fresh output, without any count given."""
+    from neko_amd import ops
+    S, H, hd, T, cap = 3, 2, 64, 3, 64
+    x = _rows(S, T, H, hd, torch.Generator().manual_seed(1)).cuda()
+    cache = ops.KV8Cache(S, H, cap, hd)
+    pos = _dev_i([-1, cap, cap - 1])
+    ops.kv8_append(cache, x[:, :, 1], x[:, :, 2], pos)
+    torch.full((S, T, H, hd), 7.0, dtype=BF16, device="cuda")          # (memory that a fresh output may come from)
+    out = ops.attn_kv8(cache, x[:, :, 0], pos)
+    assert int(out[:2].count_nonzero()) == 0 and int(out[2, 1:].count_nonzero()) == 0 and bool(torch.isfinite(out).all())
+    assert int(out[2, 0].count_nonzero()) > 0

@@ -178,3 +178,14 @@ def test_distillation_refusals():
         m.forward(_batch(), compute_loss=True, teacher=engine.Teacher(t.values[:-1], t.indices[:-1]))
     with pytest.raises(ValueError, match="compute_loss"):
         m.forward(_batch(), teacher=t)
+
+
+def test_speculative_ends_on_logits_that_are_no_numbers():
+    m, draft = _policy(seed=0), _policy(seed=5, layers=1)
+    with torch.no_grad():
+        dict(m.named_parameters())["predict_token.weight"].fill_(float("nan"))
+    m._flat.ensure_shadow()
+    with pytest.raises(RuntimeError, match="no number"):
+        m.predict_text_speculative(_prompt(20), draft, max_length=4)
+    with pytest.raises(ValueError, match="max_length"):
+        m.predict_text_speculative(_prompt(20), draft, max_length=0)
