@@ -379,7 +379,7 @@ int neko_patch_pos_add_bwd_sorted(const float* dout, const int* hkeys_sorted, co
  *   the split of the key axis and changes no result beyond rounding.  ws: neko_attn_kv8_ws_floats(..) floats (may be 0), private to the call.
  * neko_verify_draft: sequence b, K + 1 rows of target logits (element (b, i, v) at b * t_sb + i * t_sr + v; fp32 or bf16), n = n_draft[b] <= K
  *   drafted tokens [B][K] (n_draft NULL: K), draft logits in the same way or NULL (the draft was certain), u [B][K], r [B] in [0, 1).
- *   With p_i, q_i the softmax at `temperature`: token i is kept while u_i q_i(x_i) < p_i(x_i); the token behind the `accepted` kept ones is the
+ *   With p_i, q_i the softmax at `temperature` (finite): token i is kept while u_i q_i(x_i) < p_i(x_i); the token behind the `accepted` kept ones is the
  *   smallest v whose cumulative weight exceeds r times the total, weights max(p - q, 0) of the first row not kept (p where nothing is left),
  *   or p of row n.  temperature 0: kept while x_i is the row's largest logit (lowest index among equals), then the row's largest.
  *   out_tokens [B][K + 1]: the kept tokens, the next one, then -1.  NaN logits count as -inf; a row without a logit above -inf keeps

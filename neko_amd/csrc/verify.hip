@@ -33,7 +33,7 @@ struct VerifyArgs {
   double* pw;         // [B][pieces][2] sums of the sampled weights: the residual's, the target's own
   Source* src; // [B]
   int B, K, V, pieces;
-  double c;           // log2(e) / tau
+  double c, low;      // log2(e) / tau; the distance from the maximum where weights end, -1000 / c
   int greedy;
 };
 
@@ -45,11 +45,12 @@ template <typename T> __device__ __forceinline__ float raw_logit(const T* p, int
 template <> __device__ __forceinline__ float raw_logit<float>(const float* p, int i) { return p[i]; }
 template <> __device__ __forceinline__ float raw_logit<bf16_t>(const bf16_t* p, int i) { return bf16_to_f32(p[i]); }
 
-// 2^x for x <= 1/2, fp64: x = n + f, the polynomial of degree 9 that interpolates 2^f at the ten Chebyshev nodes of [-1/2, 1/2] (relative error
-// 2e-14), n added to the exponent field.  Adding 1.5 2^52 leaves n in the sum's low word: no conversion and no ldexp.  pow2_64: 0 below -1000, for -inf and for NaN
-__device__ __forceinline__ double pow2_64_above_1000(double x) {
+// 2^(d c) for -1000 <= d c <= 1/2, fp64: d c = n + f, the polynomial of degree 9 that interpolates 2^f at the ten Chebyshev nodes of [-1/2, 1/2]
+// (relative error 2e-14), n added to the exponent field.  Adding 1.5 2^52 leaves n in the sum's low word: no conversion and no ldexp; and the product
+// is part of both multiply-adds, so it is never rounded
+__device__ __forceinline__ double pow2_64(double d, double c) {
   constexpr double MAGIC = 6755399441055744.0;
-  const double y = x + MAGIC, f = x - (y - MAGIC);
+  const double y = fma(d, c, MAGIC), f = fma(d, c, MAGIC - y);
   double p = 1.02059054137655955e-07;
   p = fma(p, f, 1.32596452448871106e-06);
   p = fma(p, f, 1.52526729248507372e-05);
@@ -62,20 +63,17 @@ __device__ __forceinline__ double pow2_64_above_1000(double x) {
   p = fma(p, f, 1.00000000000001354e+00);
   return __hiloint2double(__double2hiint(p) + (__double2loint(y) << 20), __double2loint(p));
 }
-__device__ __forceinline__ double pow2_64(double x) {
-  const double r = pow2_64_above_1000(x);
-  return x > -1000.0 ? r : 0.0;
-}
 // weight of logit l under the maximum m, c = log2(e) / tau: 2^((l - m) c), exactly 1 for the maximum at any temperature (c l - c m in one multiply-add
-// is off by the rounding of c m); an infinite maximum shares the mass among its equals
+// is off by the rounding of c m), 0 below 2^-1000; an infinite maximum shares the mass among its equals
 struct Weigh {
-  double c;
+  double c, low;
   float m;
   bool inf;
-  __device__ __forceinline__ Weigh(float m_, double c_) : c(c_), m(m_), inf(m_ == INFINITY || m_ == -INFINITY) {}
+  __device__ __forceinline__ Weigh(float m_, const VerifyArgs& a) : c(a.c), low(a.low), m(m_), inf(m_ == INFINITY || m_ == -INFINITY) {}
   __device__ __forceinline__ double operator()(float l) const {
     if (__builtin_expect(inf, 0)) return l == m && m == INFINITY ? 1.0 : 0.0;
-    return pow2_64(((double)l - (double)m) * c);
+    const double d = (double)l - (double)m;
+    return d > low ? pow2_64(d, c) : 0.0;
   }
 };
 __device__ __forceinline__ double wave_sum64(double v) {
@@ -94,7 +92,7 @@ __device__ __forceinline__ double wave_scan64(double v, int lane) {       // inc
 __device__ __forceinline__ int drafted(const VerifyArgs& a, int b) { return min(max(a.n_draft ? a.n_draft[b] : a.K, 0), a.K); }
 
 // ---- launch 1: every row piece -> maximum and sum (or the maximum's index) ----
-// Bound by the vector unit: an element costs 21 instructions (16 of them fp64), so everything else stays out of the loop: whole pieces load and
+// Bound by the vector unit: an element costs 20 instructions (15 of them fp64), so everything else stays out of the loop: whole pieces load and
 // compare without bounds, and a NaN needs no test (the maximum ignores it, the lower bound of the exponent turns it into nothing).
 template <typename T, bool GREEDY>
 __global__ __launch_bounds__(VT) void verify_rows_kernel(VerifyArgs a) {
@@ -151,10 +149,10 @@ __global__ __launch_bounds__(VT) void verify_rows_kernel(VerifyArgs a) {
 #pragma unroll
     for (int e = 0; e < VE; ++e) s += x[e] == bm && bm == INFINITY ? 1.0 : 0.0;
   } else {
-    const double dm = (double)bm;
+    const double dm = (double)bm, low = a.low;
     // exponents stop at -1000: 2^-1000 beside the 1 of the maximum is nothing, and the exponent field does not run over
 #pragma unroll
-    for (int e = 0; e < VE; ++e) s += pow2_64_above_1000(fmax(((double)x[e] - dm) * a.c, -1000.0));
+    for (int e = 0; e < VE; ++e) s += pow2_64(fmax((double)x[e] - dm, low), a.c);
   }
   s = wave_sum64(s);
   if (lane == 0) ss[wave] = s;
@@ -202,7 +200,7 @@ __global__ __launch_bounds__(VT) void verify_accept_kernel(VerifyArgs a) {
     for (int p = lane & 15; p < a.pieces; p += 16) m = fmaxf(m, a.pm[o + p]);
 #pragma unroll
     for (int d = 1; d < 16; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
-    const Weigh w(m, a.c);
+    const Weigh w(m, a);
     double s = 0.0;
     for (int p = lane & 15; p < a.pieces; p += 16) s += a.ps[o + p] * w(a.pm[o + p]);
 #pragma unroll
@@ -213,8 +211,8 @@ __global__ __launch_bounds__(VT) void verify_accept_kernel(VerifyArgs a) {
   if (wave == 0) {                                                    // lane i judges draft i
     bool ok = false;
     if (lane < n && x >= 0 && x < a.V) {
-      const double p = Weigh(row_m[lane], a.c)(lx) / row_s[lane];
-      const double q = a.draft ? Weigh(row_m[n + 1 + lane], a.c)(qx) / row_s[n + 1 + lane] : 1.0;
+      const double p = Weigh(row_m[lane], a)(lx) / row_s[lane];
+      const double q = a.draft ? Weigh(row_m[n + 1 + lane], a)(qx) / row_s[n + 1 + lane] : 1.0;
       ok = (double)u * q < p;
     }
     const unsigned long long bad = ~__builtin_amdgcn_ballot_w64(ok);
@@ -251,7 +249,7 @@ __global__ __launch_bounds__(VT) void verify_accept_kernel(VerifyArgs a) {
     lp[e] = logit<T>(zp, c);
     lq[e] = logit<T>(zq, c);
   }
-  const Weigh wp(src.mp, a.c), wq(src.mq, a.c);
+  const Weigh wp(src.mp, a), wq(src.mq, a);
   double sr = 0.0, so = 0.0;
 #pragma unroll
   for (int e = 0; e < VE; ++e) {
@@ -347,7 +345,7 @@ __global__ __launch_bounds__(VT) void verify_sample_kernel(VerifyArgs a) {
   }
   const T* zp = (const T*)a.target + a.t_sb * b + a.t_sr * kept;
   const T* zq = src.has_q ? (const T*)a.draft + a.d_sb * b + a.d_sr * kept : zp;
-  const Weigh wp(src.mp, a.c), wq(src.mq, a.c);
+  const Weigh wp(src.mp, a), wq(src.mq, a);
   float lp[VE], lq[VE];
 #pragma unroll
   for (int e = 0; e < VE; ++e) {
@@ -418,7 +416,7 @@ int neko_verify_draft_impl(const void* target, long t_sb, long t_sr, const void*
                            const long long* tokens, const float* u, const float* r, const int* n_draft, float temperature, int* accepted,
                            long long* out, void* ws, long ws_bytes, hipStream_t s) {
   if (!target || !tokens || !accepted || !out || !ws || B <= 0 || K <= 0 || V <= 0) return NEKO_ERR_ARG;
-  if (!(temperature >= 0.f) || (temperature > 0.f && (!u || !r))) return NEKO_ERR_ARG;
+  if (!(temperature >= 0.f && temperature <= 3.402823466e38f) || (temperature > 0.f && (!u || !r))) return NEKO_ERR_ARG;
   if (K > MAXK - 1 || B > 65535 || V > (1 << 30)) return NEKO_ERR_UNSUPPORTED;
   if ((uintptr_t)ws & 7 || ws_bytes < neko_verify_draft_ws_bytes_impl(B, K, V)) return NEKO_ERR_ARG;
   VerifyArgs a{};
@@ -432,5 +430,6 @@ int neko_verify_draft_impl(const void* target, long t_sb, long t_sr, const void*
   a.pm = (float*)(a.src + B);
   a.greedy = temperature == 0.f;
   a.c = a.greedy ? 1.0 : 1.4426950408889634074 / (double)temperature;
+  a.low = -1000.0 / a.c;
   return is_bf16 ? launch<bf16_t>(a, s) : launch<float>(a, s);
 }

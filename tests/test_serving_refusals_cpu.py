@@ -123,6 +123,10 @@ def test_distill_refuses_shared_rows(bad):
     assert _rc("neko_distill_topk", {**DISTILL, "R": 4, **bad}.values()) == -1
 
 
+def test_verify_refuses_an_infinite_temperature():
+    assert _rc("neko_verify_draft", {**VERIFY, "temperature": float("inf")}.values()) == -1
+
+
 def test_verify_refuses_long_rows():
     assert _rc("neko_verify_draft", {**VERIFY, "V": (1 << 30) + 1, "ws_bytes": 1 << 40}.values()) == -2
     assert _lib.load().neko_verify_draft_ws_bytes(1, 1, 2 ** 31 - 1) > 0
