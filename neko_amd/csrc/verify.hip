@@ -12,11 +12,17 @@
 // Reads (2 K + 1) V logits once (HBM), then the two rows that are sampled from again (last-level cache).  Three launches: row pieces ->
 // (maximum, sum); acceptance, redone by every workgroup from the pieces, and the sampled weights' sum per piece; the piece that holds the
 // border and the token in it.  tau = 0 needs two.
+// 64 sequences of seven drafts over 52305 fp32 logits: 60 us, of them 34 for the one pass over 201 MB (5.9 TB/s out of the last-level cache, the fp64
+// units at three quarters of their rate); a single sequence is three launches' latency.
 #include "neko_kernels.h"
 
 namespace {
 
-constexpr int VT = 256, VE = 16, PIECE = VT * VE;      // 4096 logits per workgroup, 16 a thread
+constexpr int PIECE = 4096;                            // logits per workgroup
+constexpr int VT = 256, VE = PIECE / VT;               // where every row is read: 16 a thread
+// where one row is sampled from, latency is all there is: 8 a thread (64 sequences of seven drafts: 15.4 + 10.9 us; 16 a thread 17.1 + 13.6,
+// 4 a thread 18.8 + 13.5)
+constexpr int ST = 512, SE = PIECE / ST;
 constexpr int MAXK = 63;                               // a lane per drafted token
 
 struct Source;
@@ -172,8 +178,8 @@ __device__ __forceinline__ double residual(float lp, float lq, int c, const Sour
 
 // ---- launch 2: acceptance (by every workgroup again, from the pieces), and the sums of the sampled weights of one piece ----
 template <typename T>
-__global__ __launch_bounds__(VT) void verify_accept_kernel(VerifyArgs a) {
-  __shared__ double ss[VT / 64][2];
+__global__ __launch_bounds__(ST) void verify_accept_kernel(VerifyArgs a) {
+  __shared__ double ss[ST / 64][2];
   __shared__ float row_m[2 * MAXK];
   __shared__ double row_s[2 * MAXK];
   __shared__ Source s_src;
@@ -193,7 +199,7 @@ __global__ __launch_bounds__(VT) void verify_accept_kernel(VerifyArgs a) {
   }
   // rows 0..n of the target, then n of the draft: sixteen lanes each
   const int nrows = a.draft ? 2 * n + 1 : n + 1;
-  for (int q = tid >> 4; q < nrows; q += VT / 16) {
+  for (int q = tid >> 4; q < nrows; q += ST / 16) {
     const int row = q <= n ? q : a.K + 1 + (q - n - 1);
     const long o = ((long)b * (2 * a.K + 1) + row) * a.pieces;
     float m = -INFINITY;
@@ -242,18 +248,18 @@ __global__ __launch_bounds__(VT) void verify_accept_kernel(VerifyArgs a) {
   const Source src = s_src;
   const T* zp = (const T*)a.target + a.t_sb * b + a.t_sr * kept;
   const T* zq = src.has_q ? (const T*)a.draft + a.d_sb * b + a.d_sr * kept : zp;
-  float lp[VE], lq[VE];
+  float lp[SE], lq[SE];
 #pragma unroll
-  for (int e = 0; e < VE; ++e) {
-    const int c = min(piece * PIECE + e * VT + tid, a.V - 1);
+  for (int e = 0; e < SE; ++e) {
+    const int c = min(piece * PIECE + e * ST + tid, a.V - 1);
     lp[e] = logit<T>(zp, c);
     lq[e] = logit<T>(zq, c);
   }
   const Weigh wp(src.mp, a), wq(src.mq, a);
   double sr = 0.0, so = 0.0;
 #pragma unroll
-  for (int e = 0; e < VE; ++e) {
-    const int c = piece * PIECE + e * VT + tid;
+  for (int e = 0; e < SE; ++e) {
+    const int c = piece * PIECE + e * ST + tid;
     double own;
     const double res = residual<T>(lp[e], lq[e], c, src, wp, wq, own);
     if (c < a.V) { sr += res; so += own; }
@@ -264,8 +270,10 @@ __global__ __launch_bounds__(VT) void verify_accept_kernel(VerifyArgs a) {
   __syncthreads();
   if (tid == 0) {
     double* w = a.pw + ((long)b * a.pieces + piece) * 2;
-    w[0] = (ss[0][0] + ss[1][0]) + (ss[2][0] + ss[3][0]);
-    w[1] = (ss[0][1] + ss[1][1]) + (ss[2][1] + ss[3][1]);
+    double t0 = 0.0, t1 = 0.0;
+    for (int i = 0; i < ST / 64; ++i) { t0 += ss[i][0]; t1 += ss[i][1]; }
+    w[0] = t0;
+    w[1] = t1;
   }
 }
 
@@ -309,9 +317,9 @@ __global__ __launch_bounds__(VT) void verify_greedy_kernel(VerifyArgs a) {
 
 // ---- launch 3: the piece that holds the border, and the token in it ----
 template <typename T>
-__global__ __launch_bounds__(VT) void verify_sample_kernel(VerifyArgs a) {
-  __shared__ double f[PIECE + PIECE / VE];                // a thread's sixteen consecutive weights, padded by one
-  __shared__ double wsum[VT / 64];
+__global__ __launch_bounds__(ST) void verify_sample_kernel(VerifyArgs a) {
+  __shared__ double f[PIECE + PIECE / SE];                // a thread's consecutive weights, padded by one
+  __shared__ double wsum[ST / 64];
   __shared__ int s_at, s_last;
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int kept = a.accepted[b];
@@ -346,35 +354,35 @@ __global__ __launch_bounds__(VT) void verify_sample_kernel(VerifyArgs a) {
   const T* zp = (const T*)a.target + a.t_sb * b + a.t_sr * kept;
   const T* zq = src.has_q ? (const T*)a.draft + a.d_sb * b + a.d_sr * kept : zp;
   const Weigh wp(src.mp, a), wq(src.mq, a);
-  float lp[VE], lq[VE];
+  float lp[SE], lq[SE];
 #pragma unroll
-  for (int e = 0; e < VE; ++e) {
-    const int c = min(piece * PIECE + e * VT + tid, a.V - 1);
+  for (int e = 0; e < SE; ++e) {
+    const int c = min(piece * PIECE + e * ST + tid, a.V - 1);
     lp[e] = logit<T>(zp, c);
     lq[e] = logit<T>(zq, c);
   }
 #pragma unroll
-  for (int e = 0; e < VE; ++e) {
-    const int i = e * VT + tid, c = piece * PIECE + i;
+  for (int e = 0; e < SE; ++e) {
+    const int i = e * ST + tid, c = piece * PIECE + i;
     double own;
     const double res = residual<T>(lp[e], lq[e], c, src, wp, wq, own);
-    f[i + i / VE] = c < a.V ? (col ? own : res) : 0.0;
+    f[i + i / SE] = c < a.V ? (col ? own : res) : 0.0;
   }
   if (tid == 0) { s_at = 0x7fffffff; s_last = -1; }
   __syncthreads();
   double sum = 0.0;
 #pragma unroll
-  for (int e = 0; e < VE; ++e) sum += f[tid * (VE + 1) + e];
+  for (int e = 0; e < SE; ++e) sum += f[tid * (SE + 1) + e];
   const double incl = wave_scan64(sum, lane);
   if (lane == 63) wsum[wave] = incl;
   __syncthreads();
   double run = before + (incl - sum);
   for (int i = 0; i < wave; ++i) run += wsum[i];
-  const int c0 = piece * PIECE + tid * VE;
+  const int c0 = piece * PIECE + tid * SE;
   int at = 0x7fffffff, last = -1;
 #pragma unroll
-  for (int e = 0; e < VE; ++e) {
-    const double x = f[tid * (VE + 1) + e];
+  for (int e = 0; e < SE; ++e) {
+    const double x = f[tid * (SE + 1) + e];
     run += x;
     if (x > 0.0) {
       last = c0 + e;
@@ -396,9 +404,9 @@ int launch(const VerifyArgs& a, hipStream_t s) {
   if (a.greedy) {
     hipLaunchKernelGGL(verify_greedy_kernel, dim3(a.B), dim3(VT), 0, s, a);
   } else {
-    hipLaunchKernelGGL((verify_accept_kernel<T>), dim3(a.pieces, a.B), dim3(VT), 0, s, a);
+    hipLaunchKernelGGL((verify_accept_kernel<T>), dim3(a.pieces, a.B), dim3(ST), 0, s, a);
     NEKO_CHECK_LAUNCH();
-    hipLaunchKernelGGL((verify_sample_kernel<T>), dim3(a.B), dim3(VT), 0, s, a);
+    hipLaunchKernelGGL((verify_sample_kernel<T>), dim3(a.B), dim3(ST), 0, s, a);
   }
   NEKO_CHECK_LAUNCH();
   return NEKO_OK;
