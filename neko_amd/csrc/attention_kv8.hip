@@ -75,7 +75,7 @@ __device__ __forceinline__ bool visible(const Sight& v, int key) {
 constexpr int KT = 64;
 
 template <int HD, int DT, int NQ, int NW>
-__global__ __launch_bounds__(NW * 64, NQ == 1 || (NQ == 2 && HD < 128) ? 2 : 1) void attn_kv8_rows_kernel(AttnArgs a) {
+__global__ __launch_bounds__(NW * 64, NQ == 1 || HD < 128 ? 2 : 1) void attn_kv8_rows_kernel(AttnArgs a) {
   constexpr int NC = HD / 16;                 // channel tiles
   constexpr int NK = HD / 32;                 // contraction steps of the scores
   constexpr int LDO = HD + 4;
@@ -312,7 +312,7 @@ __device__ __forceinline__ int kimg(int row, int piece) {
 }
 
 template <int HD, int DT, int NW>
-__global__ __launch_bounds__(NW * 64) void attn_kv8_tile_kernel(AttnArgs a) {
+__global__ __launch_bounds__(NW * 64, 2) void attn_kv8_tile_kernel(AttnArgs a) {
   constexpr int NC = HD / 32, NK = HD / 16;
   constexpr int IMG = KT * HD * 2;                        // bytes of one image
   constexpr int UNITS = KT * HD / 16;                     // 16-byte pieces of K, and of V, in a tile
@@ -612,37 +612,36 @@ __global__ __launch_bounds__(256) void attn_kv8_merge_kernel(AttnArgs a, int row
   *reinterpret_cast<uint2*>(a.out + a.o_ss * s + a.o_st * t + (long)(h * a.G + gq) * HD + c4) = pk;
 }
 
-// How a call is cut.  More than 64 rows a key head go through LDS tiles (a row tile of 128 or 256); up to 64 stay in the register kernel, 16 / 32 /
-// 64 rows a wave.  The key axis is cut into the number of splits with the least estimated time: rounds of resident workgroups x (64-key tiles of
-// the longest wave + a constant for start and end) + the merge of the partial results.  `keys`: the most a row can see.
-struct Plan { int tiled, nq, nw, rt, rtiles, splits; };
+// How a call is cut: the kernel, its row tile and the number of splits of the key axis with the least estimated time
+//   launch + (fixed + step * (64-key tiles of the longest wave)) * (1 + crowd * (workgroups per CU - 1)) + the merge of the partial results, if any
+// in us, fitted (least squares of the logarithms) to 2000 measured calls: 8, 64, 256 key heads x sequences, 500 - 4000 keys, 16 - 384 rows, 1 - 32
+// splits, each of the four kernels.  The cut taken is 2 % slower on average than the best measured one; a choice by the number of rows alone was
+// 19 %, even with the best splits.  Both sides, 4000 keys: 64 rows of one sequence, 8 heads of 128: 13.4 us with 16 rows a wave, 17.9 with 32,
+// 20.6 through LDS; 32 rows, 64 heads of 64: 18.3 | 19.1 | 22.9; 128 rows, 64 heads of 128: 75 | 73 | 39; 256 rows, 256 heads of 128: 164 with 128
+// rows a workgroup, 145 with 256.
+// Up to 64 rows stay in the register kernel, which keeps probabilities to 16 bits.
+struct Plan { int rt, rtiles, splits; };
+struct Cost { float fixed, step, crowd; };
+constexpr Cost COST[3][4] = {{{0.12f, 1.34f, 1.0f}, {0.64f, 1.67f, 0.60f}, {1.68f, 0.77f, 0.42f}, {1.79f, 0.97f, 0.60f}},       // hd = 32
+                             {{0.43f, 2.25f, 1.0f}, {0.79f, 2.09f, 0.78f}, {2.15f, 0.99f, 0.37f}, {1.28f, 1.24f, 1.0f}},        // 64
+                             {{0.0f, 4.36f, 1.0f}, {2.39f, 3.96f, 1.0f}, {3.17f, 1.49f, 0.41f}, {1.19f, 1.87f, 1.0f}}};         // 128
 Plan plan_of(int S, int H, int hd, int rows, int keys) {
-  Plan p;
-  p.tiled = rows > 64;
-  if (p.tiled) {
-    p.nq = 0;
-    p.nw = rows <= 128 ? 4 : 8;
-    p.rt = 32 * p.nw;
-  } else {
-    p.nq = rows <= 16 ? 1 : rows <= 32 || hd == 128 ? 2 : 4;
-    p.nw = p.nq == 1 ? 8 : 4;
-    p.rt = 16 * p.nq;
-  }
-  p.rtiles = (rows + p.rt - 1) / p.rt;
-  const long base = (long)S * H * p.rtiles;
-  const int tiles = (keys + KT - 1) / KT;
-  const int per_wg = p.tiled ? 1 : p.nw;               // key tiles a workgroup works on at a time
-  const long slots = 256L * (p.tiled ? (hd == 128 ? 1 : 2) : p.nq == 1 ? (hd == 128 ? 1 : 2) : (p.nq == 2 && hd < 128 ? 2 : 1));
-  const int fixed = p.tiled ? 4 : 2;
-  int best = 1;
-  double best_t = 0;
-  for (int sp = 1; sp <= 64 && (sp == 1 || (sp - 1) * per_wg < tiles); ++sp) {
-    const long rounds = (base * sp + slots - 1) / slots;
-    const int per = (tiles + sp - 1) / sp;
-    const double t = (double)rounds * ((per + per_wg - 1) / per_wg + fixed) + (sp > 1 ? 2.0 + 0.1 * sp : 0.0);
-    if (sp == 1 || t < best_t * 0.97) { best = sp; best_t = t; }
-  }
-  p.splits = best;
+  constexpr int RT[4] = {16, 32, 128, 256}, PER_WG[4] = {8, 4, 1, 1};       // rows of a workgroup; key tiles it works on at a time
+  constexpr int SPLITS[12] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
+  const int tiles = (keys + KT - 1) / KT, kernels = rows <= 64 ? 2 : 4;
+  Plan p{};
+  float best = 0.f;
+  for (const int sp : SPLITS)
+    for (int v = 0; v < kernels; ++v) {
+      if (sp > 1 && (sp - 1) * PER_WG[v] >= tiles) continue;
+      const Cost& c = COST[hd == 32 ? 0 : hd == 64 ? 1 : 2][v];
+      const int rtiles = (rows + RT[v] - 1) / RT[v];
+      const long wgs = (long)S * H * rtiles * sp;
+      const int steps = ((tiles + sp - 1) / sp + PER_WG[v] - 1) / PER_WG[v];
+      float t = (c.fixed + c.step * steps) * (1.0f + c.crowd * ((wgs + 255) / 256 - 1));
+      if (sp > 1) t += 2.29f + 0.27f * sp + 0.15e-6f * 4 * (hd + 2) * wgs * RT[v];
+      if (best == 0.f || t < best * 0.97f) { best = t; p = Plan{RT[v], rtiles, sp}; }
+    }
   return p;
 }
 int keys_of(int cap, int T, int window, int sinks, int max_len) {
@@ -655,11 +654,10 @@ template <int HD, int DT>
 int launch_rows(const AttnArgs& a, const Plan& p, hipStream_t s) {
   const dim3 grid((unsigned)(p.splits * p.rtiles), a.H, a.S);
   const dim3 flat((unsigned)(p.splits * p.rtiles) * a.H * a.S);
-  if (p.tiled && p.nw == 4) hipLaunchKernelGGL((attn_kv8_tile_kernel<HD, DT, 4>), flat, dim3(256), 0, s, a);
-  else if (p.tiled) hipLaunchKernelGGL((attn_kv8_tile_kernel<HD, DT, 8>), flat, dim3(512), 0, s, a);
-  else if (p.nq == 1) hipLaunchKernelGGL((attn_kv8_rows_kernel<HD, DT, 1, 8>), grid, dim3(512), 0, s, a);
-  else if (p.nq == 2) hipLaunchKernelGGL((attn_kv8_rows_kernel<HD, DT, 2, 4>), grid, dim3(256), 0, s, a);
-  else if constexpr (HD < 128) hipLaunchKernelGGL((attn_kv8_rows_kernel<HD, DT, 4, 4>), grid, dim3(256), 0, s, a);
+  if (p.rt == 256) hipLaunchKernelGGL((attn_kv8_tile_kernel<HD, DT, 8>), flat, dim3(512), 0, s, a);
+  else if (p.rt == 128) hipLaunchKernelGGL((attn_kv8_tile_kernel<HD, DT, 4>), flat, dim3(256), 0, s, a);
+  else if (p.rt == 16) hipLaunchKernelGGL((attn_kv8_rows_kernel<HD, DT, 1, 8>), grid, dim3(512), 0, s, a);
+  else hipLaunchKernelGGL((attn_kv8_rows_kernel<HD, DT, 2, 4>), grid, dim3(256), 0, s, a);
   NEKO_CHECK_LAUNCH();
   if (p.splits > 1) {
     const int rows = a.T * a.G, per = 256 / (HD / 4);
