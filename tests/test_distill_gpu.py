@@ -179,3 +179,15 @@ def test_distill_cold(tau, dtype):
         # in the exponent; fp32: four products
         rel = 2.0 ** -8 + 2.0 ** -18 if dtype == torch.bfloat16 else 4 * 2.0 ** -24 + 2.0 ** -22
         assert bool(((dz[r, :V].double() - want).abs() <= rel * want.abs()).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hard", [0.0, 0.4])
+@pytest.mark.parametrize("pieces", [257, 513, 1300, 2100, 3100, 4097, 4700, 5500, 6100, 7100, 7700, 9001, 11000])
+def test_distill_every_row_length(pieces, hard, dtype):
+    """Rows of that many 16-byte pieces, the last one partly filled: one per number of rounds a row can take."""
+    n = 8 if dtype == torch.bfloat16 else 4
+    V = pieces * n - 3
+    z, Vpad, tv, ti, w, y = _case(2, V, 9, dtype, seed=pieces)
+    assert Vpad == pieces * n
+    _check(z, V, Vpad, tv, ti, w, y, 2.0, hard)
