@@ -72,6 +72,9 @@ __device__ __forceinline__ bool visible(const Sight& v, int key) {
 // 16 x 16 tile); the keys a matrix row stands for are chosen so that a lane's 16 scores of a 64-key tile are 16 CONSECUTIVE positions:
 // matrix row r of tile t is key 16 (r / 4) + 4 t + r % 4.  They are then, as they stand, the operand of O^T = V^T P^T whose other
 // operand is one 16-byte load of V's transposed tile, and they share one block scale.
+// Bound by the cache's bytes where there are many: one token for each of 32 sequences of up to 8192 keys, 16 heads of 128 in int8: 139 us, 5.1 TB/s
+// (a copy: 5.2); by the latency of positions -> queries and keys -> products -> the meeting of the waves where there are few: 7 us for 24 heads
+// of 32 over 1000 keys.
 constexpr int KT = 64;
 
 template <int HD, int DT, int NQ, int NW>
@@ -301,7 +304,8 @@ __global__ __launch_bounds__(NW * 64, NQ == 1 || HD < 128 ? 2 : 1) void attn_kv8
 // factor), so the common step takes no maximum.  Probabilities are rounded to bf16 once, and the sums are of the rounded ones: their errors are
 // independent and average out like the values' own (measured 1.0-1.4 x the error of the rounded output); a second product for their low parts
 // would cost 50 % of the matrix work.
-// 4 sequences x 16 heads of 128, 1024 queries over 2976-4000 keys: 140 us (0.83 PFLOP/s; 156 with a maximum a tile).  The products and their
+// 4 sequences x 16 heads of 128, 1024 queries over 2976-4000 keys: 126 us in a row of calls (0.93 PFLOP/s), 140 one at a time (156 with a maximum
+// a tile).  The products and their
 // operand reads alone take 53 us, with the staging 62: what binds it are the vector instructions of the softmax (130 a tile and wave), which two
 // waves of a SIMD in the same phase do not hide behind each other's products.  Opposite phases for the two halves of the workgroup, a barrier
 // between the phases, took 151; softmax of one tile beside the products of another within a wave 155.

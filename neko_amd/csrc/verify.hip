@@ -12,15 +12,15 @@
 // Reads (2 K + 1) V logits once (HBM), then the two rows that are sampled from again (last-level cache).  Three launches: row pieces ->
 // (maximum, sum); acceptance, redone by every workgroup from the pieces, and the sampled weights' sum per piece; the piece that holds the
 // border and the token in it.  tau = 0 needs two.
-// 64 sequences of seven drafts over 52305 fp32 logits: 60 us, of them 34 for the one pass over 201 MB (5.9 TB/s out of the last-level cache, the fp64
-// units at three quarters of their rate); a single sequence is three launches' latency.
+// 64 sequences of three to seven drafts over 52305 fp32 logits: 58 us, of them 34 for the one pass over 147 MB (4.3 TB/s; the fp64 units at half
+// their rate); a single sequence is three launches' latency.
 #include "neko_kernels.h"
 
 namespace {
 
 constexpr int PIECE = 4096;                            // logits per workgroup
 constexpr int VT = 256, VE = PIECE / VT;               // where every row is read: 16 a thread
-// where one row is sampled from, latency is all there is: 8 a thread (64 sequences of seven drafts: 15.4 + 10.9 us; 16 a thread 17.1 + 13.6,
+// where one row is sampled from, latency is all there is: 8 a thread (64 sequences of three to seven drafts: 15.4 + 10.9 us; 16 a thread 17.1 + 13.6,
 // 4 a thread 18.8 + 13.5)
 constexpr int ST = 512, SE = PIECE / ST;
 constexpr int MAXK = 63;                               // a lane per drafted token
