@@ -335,3 +335,90 @@ def test_attn_fresh_output_is_defined():
     out = ops.attn_kv8(cache, x[:, :, 0], pos)
     assert int(out[:2].count_nonzero()) == 0 and int(out[2, 1:].count_nonzero()) == 0 and bool(torch.isfinite(out).all())
     assert int(out[2, 0].count_nonzero()) > 0
+
+
+def _attention_by_heads(q, k, v, pos, n, start, window, sinks, scale, out):
+    """serving_ref.attention, all rows of a head at once: q [S, T, Hq, hd], k / v fp64 [S, H, cap, hd]."""
+    S, T, HQ, hd = q.shape
+    H, cap = k.shape[1], k.shape[2]
+    G = HQ // H
+    want, absv, big = out.double().clone(), torch.zeros(out.shape, dtype=torch.float64), torch.zeros(S, T, HQ, 1, dtype=torch.float64)
+    t = torch.arange(cap)
+    for s in range(S):
+        m = min(n[s], T, cap - pos[s]) if 0 <= pos[s] < cap else 0
+        if m <= 0:
+            continue
+        p = pos[s] + torch.arange(m)[:, None]
+        seen = (t <= p) & (t >= start[s])
+        if window:
+            seen &= (t > p - window) | (t < start[s] + sinks)
+        seen = seen[None, None]                                              # [1, 1, m, cap]
+        qq = q[s, :m].double().view(m, H, G, hd).permute(1, 2, 0, 3)           # [H, G, m, hd]
+        sc = (qq @ k[s].transpose(1, 2)[:, None]) * scale
+        sc = sc.masked_fill(~seen, -float("inf"))
+        w = torch.nan_to_num(torch.softmax(sc, -1), nan=0.0)
+        put = lambda x: x.permute(2, 0, 1, 3).reshape(m, HQ, -1)
+        want[s, :m] = put(w @ v[s][:, None])
+        absv[s, :m] = put(w @ v[s].abs()[:, None])
+        big[s, :m] = put(((qq.abs() @ k[s].abs().transpose(1, 2)[:, None]) * scale).masked_fill(~seen, 0.0).amax(-1, keepdim=True))
+    return want, absv, big
+
+
+# heads and rows that take each of the kernels: 16 and 32 rows a wave, 128 and 256 rows through LDS, with one split of the keys and several
+@pytest.mark.parametrize("hd,S,H,G,T,cap", [(32, 16, 16, 1, 100, 320), (32, 16, 16, 1, 130, 320), (32, 8, 8, 3, 100, 320), (32, 8, 8, 1, 520, 1024), (64, 16, 16, 1, 20, 320),
+                                            (64, 8, 8, 1, 100, 320), (64, 8, 8, 1, 130, 320), (64, 8, 8, 1, 130, 1024), (64, 8, 8, 2, 150, 1024), (64, 16, 16, 1, 100, 320),
+                                            (128, 8, 8, 1, 20, 1024), (128, 8, 8, 1, 100, 1024), (128, 8, 8, 1, 130, 1024), (128, 8, 8, 4, 130, 1024), (128, 2, 4, 1, 520, 1024)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (150, 70)])
+def test_attn_many_heads(hd, S, H, G, T, cap, window, sinks):
+    from neko_amd import ops
+    g = torch.Generator().manual_seed(hd + T + window)
+    dtype, block = (E4, 16) if (T + window) % 4 else (I8, 64)
+    pos = [int(x) for x in torch.randint(0, cap - T // 2, (S,), generator=g)]
+    n = [int(x) for x in torch.randint(0, T + 1, (S,), generator=g)]
+    n[0], pos[0], n[1], pos[1] = T, cap - T, T, 0
+    end = [min(cap, p + m) if m else 0 for p, m in zip(pos, n)]
+    start = [int(x) for x in (torch.rand(S, generator=g) * 0.7 * torch.tensor(end))]
+    start[0] = 0
+    start[1] = min(T // 3, cap - 1)                                            # its first rows see nothing
+    cache = ops.KV8Cache(S, H, cap, hd, dtype=dtype, block=block)
+    cache.k.view(torch.uint8).fill_(0x7f)                                      # outside the rows: NaN or large codes under wild scales
+    cache.v.view(torch.uint8).fill_(0x7f)
+    cache.k_scale.fill_(float("inf"))
+    cache.v_scale.fill_(float("nan"))
+    x = _rows(S, cap, H, hd, g, spread=0.4).cuda()
+    ops.kv8_append(cache, x[:, :, 1], x[:, :, 2], _dev_i([0] * S), n_new=_dev_i(end))
+    k, v = (a.cpu().double().transpose(1, 2) for a in ops.kv8_read(cache, _dev_i(end), cap))
+    q = torch.randn(S, T, H * G, hd, generator=g).to(BF16)
+    out0 = torch.full((S, T, H * G, hd), 7.0, dtype=BF16)
+    out = out0.cuda()
+    ops.attn_kv8(cache, q.cuda(), _dev_i(pos), n_new=_dev_i(n), start=_dev_i(start), window=window, sinks=sinks, out=out)
+    want, absv, big = _attention_by_heads(q, k, v, pos, n, start, window, sinks, hd ** -0.5, out0)
+    p_round = 2.0 ** -8 if T * G > 64 else 2.0 ** -16                          # tolerances as in _attn_case
+    tol = 2.0 ** -8 * want.abs() + (p_round + 2 * hd * 2.0 ** -23 * big + cap * 2.0 ** -23 + 2.0 ** -21) * absv
+    err = (out.cpu().double() - want).abs()
+    assert bool((err <= tol).all()), float((err - tol).max())
+    for s in range(S):
+        assert torch.equal(out[s, n[s]:].cpu(), out0[s, n[s]:])
+
+
+@pytest.mark.parametrize("hd,S,H,T,cap", [(32, 16, 16, 100, 320), (32, 16, 16, 130, 320), (128, 8, 8, 130, 1024)])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_attn_rising_scores_many_heads(hd, S, H, T, cap, sign):
+    """test_attn_rising_and_falling_scores through LDS tiles, where the running reference moves only when probabilities outgrow 2^40."""
+    from neko_amd import ops
+    g = torch.Generator().manual_seed(T + hd)
+    u = torch.randn(S, 1, H, hd, generator=g)
+    ramp = sign * torch.linspace(-60.0, 60.0, cap).view(1, cap, 1, 1)
+    k = (ramp * u / hd ** 0.5 + 0.1 * torch.randn(S, cap, H, hd, generator=g)).to(BF16)
+    v = torch.randn(S, cap, H, hd, generator=g).to(BF16)
+    q = (8.0 * u + 0.1 * torch.randn(S, T, H, hd, generator=g)).to(BF16)
+    cache = ops.KV8Cache(S, H, cap, hd, dtype=E4, block=16)
+    ops.kv8_append(cache, k.cuda(), v.cuda(), _dev_i([0] * S))
+    pos = [cap - T] * S
+    got = ops.attn_kv8(cache, q.cuda(), _dev_i(pos))
+    kk, vv = (t.cpu().double().transpose(1, 2) for t in ops.kv8_read(cache, _dev_i([cap] * S), cap))
+    want, absv, big = _attention_by_heads(q, kk, vv, pos, [T] * S, [0] * S, 0, 0, hd ** -0.5, torch.zeros(S, T, H, hd))
+    # as in test_attn_rising_and_falling_scores
+    tol = 2.0 ** -8 * want.abs() + (2.0 ** -8 + (2 * hd + 8) * 2.0 ** -23 * big + cap * 2.0 ** -23 + 2.0 ** -21) * absv
+    err = (got.cpu().double() - want).abs()
+    assert bool((err <= tol).all()), float((err - tol).max())
