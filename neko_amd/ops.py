@@ -654,7 +654,7 @@ class KV8Cache:
     per block of 16 / 32 / 64 positions and head.  The cache does not know how much of it is filled: positions are arguments of kv8_append,
     kv8_read and attn_kv8 (device tensors, so that a captured step can advance them)."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "nseq", "heads", "cap", "hd", "block", "dtype", "device", "_args")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "nseq", "heads", "cap", "hd", "block", "dtype", "_args")
 
     def __init__(self, nseq: int, heads: int, cap: int, hd: int, dtype=torch.float8_e4m3fn, block: int = 32, device="cuda"):
         assert dtype in _KV8_DTYPES, f"cache dtype must be one of {list(_KV8_DTYPES)}, got {dtype}"
@@ -666,28 +666,31 @@ class KV8Cache:
 
     def _set(self, k, v, k_scale, v_scale, S, H, cap, hd, block):
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.nseq, self.heads, self.cap, self.hd, self.block = S, H, cap, hd, block
-        self.dtype, self.device = k.dtype, k.device
+        self.nseq, self.heads, self.cap, self.hd, self.block, self.dtype = S, H, cap, hd, block, k.dtype
         # the leading arguments of every entry point of the cache
         self._args = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), _KV8_DTYPES[k.dtype], S, H, cap, hd, block)
+
+    @property
+    def device(self) -> torch.device:
+        return self.k.device
 
     @classmethod
     def from_tensors(cls, k, v, k_scale, v_scale) -> "KV8Cache":
         """A cache over tensors that the caller holds (no copy): k, v, k_scale, v_scale as in the class description, contiguous."""
-        dt, dev = k.dtype, k.device
-        assert dt in _KV8_DTYPES and v.dtype is dt and k.dim() == 4 and k_scale.dim() == 3, "k [nseq, heads, cap, hd] and v in e4m3 or int8"
+        dt, dev, sc = k.dtype, k.get_device(), k_scale.shape
+        assert dt in _KV8_DTYPES and v.dtype is dt and k.dim() == 4 and len(sc) == 3, "k [nseq, heads, cap, hd] and v in e4m3 or int8"
         S, H, cap, hd = k.shape
-        nb = k_scale.shape[2]
+        nb = sc[2]
         assert cap > 0 and cap % 64 == 0 and hd in (32, 64, 128), "cap must be a positive multiple of 64, hd 32 / 64 / 128"
         assert nb > 0 and cap % nb == 0 and cap // nb in (16, 32, 64), "one scale per 16 / 32 / 64 positions"
         assert v.shape == (S, H, cap // 16, hd, 16), f"v must be {(S, H, cap // 16, hd, 16)}, got {tuple(v.shape)}"
-        assert k_scale.shape == v_scale.shape == (S, H, nb), "scales must be [nseq, heads, cap / block]"
+        assert sc == (S, H, nb) and v_scale.shape == sc, "scales must be [nseq, heads, cap / block]"
         assert k_scale.dtype is _F32 and v_scale.dtype is _F32, "scales must be float32"
         assert k.is_contiguous() and v.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous(), "cache tensors must be contiguous"
-        assert v.device == dev and k_scale.device == dev and v_scale.device == dev, "cache tensors must be on one device"
-        assert (k.data_ptr() | v.data_ptr()) % 16 == 0, "cache tensors must be 16-byte aligned"
+        assert dev == v.get_device() == k_scale.get_device() == v_scale.get_device(), "cache tensors must be on one device"
         c = cls.__new__(cls)
         c._set(k, v, k_scale, v_scale, S, H, cap, hd, cap // nb)
+        assert (c._args[0] | c._args[1]) % 16 == 0, "cache tensors must be 16-byte aligned"
         return c
 
     def row_strides(self, x: torch.Tensor, heads: int, name: str, dev: int):
