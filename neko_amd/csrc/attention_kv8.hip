@@ -308,7 +308,7 @@ __global__ __launch_bounds__(NW * 64, NQ == 1 || HD < 128 ? 2 : 1) void attn_kv8
 // a tile).  The products and their operand reads alone take 53 us, with the staging 62: what binds it are
 // the vector instructions of the softmax (130 a tile and wave), which two waves of a SIMD in the same phase do not hide behind each other's
 // products.  Opposite phases for the two halves of the workgroup, a barrier between the phases, took 151; softmax of one tile beside the products
-// of another within a wave 155.
+// of another within a wave 155, and so with 64 rows a wave, one wave per SIMD, 176.
 template <int HD>
 __device__ __forceinline__ int kimg(int row, int piece) {
   constexpr int PC = HD / 8, SH = HD == 128 ? 0 : HD == 64 ? 1 : 2;
