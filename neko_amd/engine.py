@@ -459,11 +459,14 @@ class KVDecoder:
 
     def __init__(self, P: StackParams, cap: int, device):
         self.P, self.cap, self.n, self.device = P, int(cap), 0, device
-        self.qkv = [torch.zeros(self.cap, 3 * P.d, dtype=BF16, device=device) for _ in P.layers]
-        self.kbias = torch.zeros(1, self.cap, dtype=F32, device=device)       # all positions real: no key bias
-        self.kstart = torch.zeros(1, dtype=torch.int32, device=device)
+        self._allocate()
         self.pos = torch.zeros(1, dtype=torch.int32, device=device)           # device-side index of the next row
         self.fast_row = P.d % 8 == 0 and 4 * P.d <= 3072                      # neko_gemv_bf16 limits (K <= 3072)
+
+    def _allocate(self) -> None:
+        self.qkv = [torch.zeros(self.cap, 3 * self.P.d, dtype=BF16, device=self.device) for _ in self.P.layers]
+        self.kbias = torch.zeros(1, self.cap, dtype=F32, device=self.device)  # all positions real: no key bias
+        self.kstart = torch.zeros(1, dtype=torch.int32, device=self.device)
 
     few_rows = 1             # most rows _few_rows takes (its attention reads their position from device memory)
 
@@ -605,12 +608,12 @@ class KV8Decoder(KVDecoder):
     few_rows = 8
 
     def __init__(self, P: StackParams, cap: int, device, dtype=torch.float8_e4m3fn, block: int = 32, window: int = 0, sinks: int = 0):
-        self.P, self.cap, self.n, self.device = P, int(cap), 0, device
-        self.window, self.sinks = int(window), int(sinks)
-        size = (self.cap + 63) // 64 * 64
-        self.caches = [ops.KV8Cache(1, P.heads, size, P.d // P.heads, dtype=dtype, block=block, device=device) for _ in P.layers]
-        self.pos = torch.zeros(1, dtype=torch.int32, device=device)           # device-side index of the next row
-        self.fast_row = P.d % 8 == 0 and 4 * P.d <= 3072                      # neko_gemv_bf16 limits (K <= 3072)
+        self.dtype, self.block, self.window, self.sinks = dtype, int(block), int(window), int(sinks)
+        super().__init__(P, cap, device)
+
+    def _allocate(self) -> None:
+        P, size = self.P, (self.cap + 63) // 64 * 64
+        self.caches = [ops.KV8Cache(1, P.heads, size, P.d // P.heads, dtype=self.dtype, block=self.block, device=self.device) for _ in P.layers]
 
     def _attend_few(self, li: int, rows: torch.Tensor, o: torch.Tensor) -> None:
         H, c = self.P.heads, self.caches[li]
