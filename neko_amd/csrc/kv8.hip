@@ -63,7 +63,7 @@ __device__ __forceinline__ float scale_of(uint32_t am) {
 }
 
 // a unit (one block of one head, K or V) on its way out: where it goes, its first position, the new positions [pc, end) (end < 0: nothing),
-// and the factor of its older codes if their grid grew (0: it did not)
+// and the factor of its older codes if their grid grew (negative: it did not; 0 is a factor, where the grids lie further apart than fp32 reaches)
 struct UnitOut { long base; int b0, pc, end; float ratio; };
 
 template <int HD, int BLOCK, int DT>
@@ -139,7 +139,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
     o.b0 = b0;
     o.pc = pc;
     o.end = act ? end : -1;
-    o.ratio = grew ? was * inv : 0.f;
+    o.ratio = grew ? was * inv : -1.f;
   }
   // codes -> the wave's image of its units, as they will lie in memory (bytes of positions that are not new: whatever they are, dropped below)
   char* mine = img[threadIdx.x >> 6];
@@ -183,7 +183,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
     // positions of the piece: [t, t + len); new ones among them: [i0, i1)
     const int t = o.b0 + (is_v ? off / (16 * HD) * 16 : off / HD), len = is_v ? 16 : 1;
     const int i0 = max(o.pc - t, 0), i1 = min(o.end - t, len);
-    const bool old = o.ratio != 0.f && t < o.pc;                    // older positions whose grid grew
+    const bool old = o.ratio >= 0.f && t < o.pc;                    // older positions whose grid grew
     if (o.end < 0 || (i0 >= i1 && !old)) continue;
     const uint4 w = *reinterpret_cast<const uint4*>(mine + u2 * US + off);
     uint32_t q[4] = {w.x, w.y, w.z, w.w};
