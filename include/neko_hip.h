@@ -374,7 +374,7 @@ int neko_patch_pos_add_bwd_sorted(const float* dout, const int* hkeys_sorted, co
  *   head (query head h * G + g reads key head h), q and out bf16 with strides as k above.  Row at position p sees t with start[s] <= t <= p and,
  *   where window > 0, t > p - window or t < start[s] + sinks (start NULL: 0).  A row that sees nothing is 0.  `scale` > 0 multiplies q . k.
  *   `out` may be q itself, rows beside q's in one buffer or memory of its own; rows that overlap otherwise are refused.  Scores are held for
- *   |scale q . k| up to 2^29.
+ *   |scale q . k| up to 2^29, values up to the largest the cache keeps (beside a value of more than 2^40, one smaller by 2^160 may count as 0).
  *   What lies in the cache outside [start, last row] never reaches the output.  max_len: host-known bound on pos + T (0: cap); it sizes
  *   the split of the key axis and changes no result beyond rounding.  ws: neko_attn_kv8_ws_floats(..) floats (may be 0), private to the call.
  * neko_verify_draft: sequence b, K + 1 rows of target logits (element (b, i, v) at b * t_sb + i * t_sr + v; fp32 or bf16), n = n_draft[b] <= K

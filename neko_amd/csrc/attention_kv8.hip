@@ -11,6 +11,11 @@
 namespace {
 
 constexpr float NEVER = -3.0e38f;       // a running maximum before any visible key (finite: no special cases)
+// Sums of probabilities x values pass fp32's end long before their quotient does: values of 1.75 2^127 are kept by the cache.  Both kernels hold the
+// values by a power of two `vref`, 1 unless a visible block's scale exceeds what the kernel's sums have room for; the quotient is formed before the
+// power is put back.  Partial results are quotients too.
+constexpr float VTOP_ROWS = 0x1p64f;    // 2^24 keys x 448 x 2^64 (probabilities at most 1)
+constexpr float VTOP_TILE = 0x1p40f;    // the same x probabilities of at most 2^40: 2^113
 
 struct AttnArgs {
   const uint8_t *k8, *v8;
@@ -19,7 +24,7 @@ struct AttnArgs {
   bf16_t* out;
   long q_ss, q_st, o_ss, o_st;
   const int *pos, *n_new, *start;
-  float *part_o, *part_ml;           // [S * H][splits][row tiles * rows per tile][hd] and [..][2]
+  float *part_o, *part_ml;           // [S * H][splits][row tiles * rows per tile][hd], quotients, and [..][2], maximum and sum
   int S, H, G, cap, T, bshift, window, sinks, splits, rtiles;
   float scale_log2e;
 };
@@ -84,6 +89,7 @@ __global__ __launch_bounds__(NW * 64, NQ == 1 || HD < 128 ? 2 : 1) void attn_kv8
   constexpr int LDO = HD + 4;
   __shared__ float sm_o[NW][16][LDO];
   __shared__ float sm_ml[NW][16][2];
+  __shared__ float sm_v[NW];
   const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4;
   const int split = blockIdx.x % a.splits, rt = blockIdx.x / a.splits;
@@ -148,6 +154,7 @@ __global__ __launch_bounds__(NW * 64, NQ == 1 || HD < 128 ? 2 : 1) void attn_kv8
     kscale = ksb[b];
     vscale = vsb[b];
   };
+  float vref = 1.0f, vinv = 1.0f;             // the wave's (uniform)
   int it = split * per + wave;
   if (it < i_end) load(tile_of(sp, it), kc, vc, ksc, vsc);
   for (; it < i_end; it += NW) {
@@ -170,6 +177,18 @@ __global__ __launch_bounds__(NW * 64, NQ == 1 || HD < 128 ? 2 : 1) void attn_kv8
       if (lo > 15 || hi < 0) { vsc = 0.f; ksc = 0.f; }
     }
     const float sc = ksc * a.scale_log2e;
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(vsc * vinv > VTOP_ROWS) != 0, 0)) {
+      float top = fmaxf(vsc, __shfl_xor(vsc, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64)) * (1.0f / VTOP_ROWS);
+      const float f = vref / top;
+#pragma unroll
+      for (int iq = 0; iq < NQ; ++iq)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) o[iq][c] *= f;
+      vref = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(top)));
+      vinv = 1.0f / vref;
+    }
+    vsc *= vinv;
     bf16x8_v pf[NQ][2], pl[NQ][2];
     f32x4 st[NQ][4];
 #pragma unroll
@@ -253,6 +272,7 @@ __global__ __launch_bounds__(NW * 64, NQ == 1 || HD < 128 ? 2 : 1) void attn_kv8
   }
 
   // the waves meet
+  if (lane == 0) sm_v[wave] = vref;
 #pragma unroll
   for (int iq = 0; iq < NQ; ++iq) {
     l[iq] += __shfl_xor(l[iq], 16, 64);
@@ -270,20 +290,25 @@ __global__ __launch_bounds__(NW * 64, NQ == 1 || HD < 128 ? 2 : 1) void attn_kv8
 #pragma unroll
       for (int w = 0; w < NW; ++w) mm = fmaxf(mm, sm_ml[w][row16][0]);
       const float ms = mm == -INFINITY ? 0.f : mm;
+      float vr = sm_v[0];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) vr = fmaxf(vr, sm_v[w]);
+      const float vri = 1.0f / vr;
       float ll = 0.f;
       f32x4 acc = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
         const float f = __builtin_amdgcn_exp2f(sm_ml[w][row16][0] - ms);
         ll = fmaf(f, sm_ml[w][row16][1], ll);
-        acc += *reinterpret_cast<const f32x4*>(&sm_o[w][row16][c4]) * f;
+        acc += *reinterpret_cast<const f32x4*>(&sm_o[w][row16][c4]) * (f * (sm_v[w] * vri));
       }
+      acc *= ll == 0.f ? 0.f : 1.0f / ll;
+      acc *= vr;
       if (a.splits == 1) {
-        const float inv = ll == 0.f ? 0.f : 1.0f / ll;
         const int t = row / a.G, gq = row - t * a.G;
         uint2 pk;
-        pk.x = pack_bf16x2(acc[0] * inv, acc[1] * inv);
-        pk.y = pack_bf16x2(acc[2] * inv, acc[3] * inv);
+        pk.x = pack_bf16x2(acc[0], acc[1]);
+        pk.y = pack_bf16x2(acc[2], acc[3]);
         *reinterpret_cast<uint2*>(a.out + a.o_ss * s + a.o_st * t + (long)(h * a.G + gq) * HD + c4) = pk;
       } else {
         const long pr = (head * a.splits + split) * ((long)a.rtiles * NQ * 16) + row;
@@ -347,6 +372,21 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_kv8_tile_kernel(AttnArgs a) {
   const int t = rc / a.G, gq = rc - t * a.G;
   const Sight sight = sight_of(a, sp, sp.p0 + t);
   const int wfirst = sp.p0 + min(w0, sp.rows - 1) / a.G, wlast = sp.p0 + min(w0 + 31, sp.rows - 1) / a.G;
+  // the power of two the values are held by: from the scales of this workgroup's blocks, every wave for itself
+  float vref = 1.0f, vinv = 1.0f;
+  {
+    const int bpt = KT >> a.bshift;                       // blocks of a tile
+    float top = 0.f;
+    for (int b = lane; b < max(n, 0) * bpt; b += 64) {
+      const int blk = tile_of(sp, i0 + b / bpt) * bpt + b % bpt, at = blk << a.bshift;
+      if (at <= sp.plast && at + (1 << a.bshift) > sp.first) top = fmaxf(top, vsb[blk]);
+    }
+    top = __uint_as_float(uni(__float_as_uint(wave_max(top))));
+    if (top > VTOP_TILE) {
+      vref = top * (1.0f / VTOP_TILE);
+      vinv = 1.0f / vref;
+    }
+  }
   bf16x8_v qf[NK];
   {
     const bf16_t* qp = a.q + a.q_ss * s + a.q_st * t + (long)(h * a.G + gq) * HD + hf * 8;
@@ -429,6 +469,10 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_kv8_tile_kernel(AttnArgs a) {
       if (UNITS % NT && u >= UNITS) break;
       uint32_t w[4] = {vst[i].x, vst[i].y, vst[i].z, vst[i].w};
       float sc8 = vss[i];
+      if (__builtin_expect(vinv != 1.0f, 0)) {            // (the conversion reads a scale's exponent only: no subnormal ones)
+        sc8 *= vinv;
+        if (sc8 < 0x1p-126f) w[0] = w[1] = w[2] = w[3] = 0;
+      }
       const int t16 = u / HD, ch = u % HD;
       if (edge) {
         const int lo = sp.first - (tk + t16 * 16), hi = sp.plast - (tk + t16 * 16);
@@ -558,16 +602,20 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_kv8_tile_kernel(AttnArgs a) {
   }
   l += __shfl_xor(l, 32, 64);
   if (row >= sp.rows) return;
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[c][i] = o[c][i] * inv * vref;
   if (a.splits == 1) {
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
     bf16_t* op = a.out + a.o_ss * s + a.o_st * t + (long)(h * a.G + gq) * HD;
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         uint2 pk;
-        pk.x = pack_bf16x2(o[c][4 * j] * inv, o[c][4 * j + 1] * inv);
-        pk.y = pack_bf16x2(o[c][4 * j + 2] * inv, o[c][4 * j + 3] * inv);
+        pk.x = pack_bf16x2(o[c][4 * j], o[c][4 * j + 1]);
+        pk.y = pack_bf16x2(o[c][4 * j + 2], o[c][4 * j + 3]);
         *reinterpret_cast<uint2*>(op + c * 32 + 8 * j + 4 * hf) = pk;
       }
   } else {
@@ -599,20 +647,21 @@ __global__ __launch_bounds__(256) void attn_kv8_merge_kernel(AttnArgs a, int row
   float mm = -INFINITY;
   for (int i = 0; i < a.splits; ++i) mm = fmaxf(mm, a.part_ml[2 * (base + (long)i * rows_pad)]);
   const float ms = mm == -INFINITY ? 0.f : mm;
+  auto share = [&](int i) {                               // split i's share of the row's sum, not yet divided by it
+    const long pr = base + (long)i * rows_pad;
+    return __builtin_amdgcn_exp2f(a.part_ml[2 * pr] - ms) * a.part_ml[2 * pr + 1];
+  };
   float ll = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < a.splits; ++i) ll += share(i);
+  const float inv = ll == 0.f ? 0.f : 1.0f / ll;
   f32x4 acc = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int i = 0; i < a.splits; ++i) {
-    const long pr = base + (long)i * rows_pad;
-    const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * pr] - ms);
-    ll = fmaf(f, a.part_ml[2 * pr + 1], ll);
-    acc += *reinterpret_cast<const f32x4*>(a.part_o + pr * HD + c4) * f;
-  }
-  const float inv = ll == 0.f ? 0.f : 1.0f / ll;
+  for (int i = 0; i < a.splits; ++i) acc += *reinterpret_cast<const f32x4*>(a.part_o + (base + (long)i * rows_pad) * HD + c4) * (share(i) * inv);
   const int t = row / a.G, gq = row - t * a.G;
   uint2 pk;
-  pk.x = pack_bf16x2(acc[0] * inv, acc[1] * inv);
-  pk.y = pack_bf16x2(acc[2] * inv, acc[3] * inv);
+  pk.x = pack_bf16x2(acc[0], acc[1]);
+  pk.y = pack_bf16x2(acc[2], acc[3]);
   *reinterpret_cast<uint2*>(a.out + a.o_ss * s + a.o_st * t + (long)(h * a.G + gq) * HD + c4) = pk;
 }
 
