@@ -474,11 +474,21 @@ class KVDecoder:
         self.n = 0
         self.pos.zero_()
 
+    def mark(self) -> None:
+        """The rows from here on may be dropped again (drafted tokens)."""
+
     def truncate(self, n: int) -> None:
         """Forget every position from n on (drafted tokens that were not kept): later rows overwrite them."""
         assert 0 <= n <= self.n, f"truncate({n}) of {self.n} positions"
         self.n = n
         self.pos.fill_(n)
+
+    def _next_rows(self, n: int) -> None:
+        """Called with the number of rows that extend is about to add."""
+
+    def _qkv_rows(self, li: int, n: int) -> torch.Tensor:
+        """Where layer li's q|k|v of the next n rows is projected to."""
+        return torch.empty(n, 3 * self.P.d, dtype=BF16, device=self.device)
 
     def _attend_few(self, li: int, rows: torch.Tensor, o: torch.Tensor) -> None:
         """o (n, d) <- attention of the newest n <= few_rows q|k|v rows at *pos; appends their keys and values."""
@@ -503,7 +513,7 @@ class KVDecoder:
         for li, lp in enumerate(P.layers):
             a1 = torch.empty(n, d, dtype=BF16, device=dev)
             ops.layernorm_fwd(x, lp.ln1_w, lp.ln1_b, y16=a1, eps=P.eps)
-            row = torch.empty(n, 3 * d, dtype=BF16, device=dev)
+            row = self._qkv_rows(li, n)
             ops.gemv(a1, lp.w_qkv, n, 3 * d, d, b_kstrided=True, bias=lp.b_qkv, out_bf16=row)
             o = torch.empty(n, d, dtype=BF16, device=dev)
             self._attend_few(li, row, o)
@@ -573,6 +583,7 @@ class KVDecoder:
         n0, T = self.n, self.n + n
         if T > self.cap:
             raise ValueError(f"KVDecoder: {T} positions exceed the capacity {self.cap}")
+        self._next_rows(n)
         if n <= self.few_rows and self.fast_row:    # the decode step proper: weight-streaming products, few-query attention
             hf16 = self._few_rows(x)                # reads / appends at *pos == n0
             self.n = T
@@ -603,7 +614,11 @@ class KV8Decoder(KVDecoder):
     """KVDecoder over an 8-bit cache (ops.KV8Cache: e4m3 or int8, a scale per block of positions and head): half the bytes of the bf16 rows'
     keys and values.  Up to eight new rows at a time take the weight-streaming step (a decode step, or the drafted tokens of a verification),
     longer extensions attend to the cache instead of recomputing every row.  window > 0: a row sees the last `window` positions and the first
-    `sinks`, so a sequence may run past the context without recomputing it (the cache then holds `cap` positions, whatever the window)."""
+    `sinks`, so a sequence may run past the context without recomputing it (the cache then holds `cap` positions, whatever the window).
+
+    Rows that enter a block together share its scale, and a larger row makes the block's older codes coarser.  Rows that may be dropped again must
+    not do that to the others, so behind mark() rows enter (and attend) one at a time, each seeing what a plain decode step would, and truncate()
+    puts the block that was open at the mark back and appends the kept rows once more: the cache is then as if the others had never been there."""
 
     few_rows = 8
 
@@ -612,19 +627,74 @@ class KV8Decoder(KVDecoder):
         super().__init__(P, cap, device)
 
     def _allocate(self) -> None:
-        P, size = self.P, (self.cap + 63) // 64 * 64
-        self.caches = [ops.KV8Cache(1, P.heads, size, P.d // P.heads, dtype=self.dtype, block=self.block, device=self.device) for _ in P.layers]
+        P, size, n = self.P, (self.cap + 63) // 64 * 64, len(self.P.layers)
+        # one cache with the layers as its sequences (what concerns all of them is one call), and a view of it for each
+        self.cache = ops.KV8Cache(n, P.heads, size, P.d // P.heads, dtype=self.dtype, block=self.block, device=self.device)
+        c = self.cache
+        self.caches = [ops.KV8Cache.from_tensors(c.k[i:i + 1], c.v[i:i + 1], c.k_scale[i:i + 1], c.v_scale[i:i + 1]) for i in range(n)]
+        self._marked, self._open, self._rows = None, None, None
+        self._steps = torch.arange(self.few_rows, dtype=torch.int32, device=self.device)
+
+    def reset(self) -> None:
+        super().reset()
+        self._marked = None
+
+    def _block_at(self, n: int):
+        """Codes and scales of every layer's block that position n lies in (views)."""
+        c, b = self.cache, n // self.block
+        t, w = b * self.block, self.block
+        return [c.k[:, :, t:t + w].view(torch.uint8), c.v[:, :, t // 16:(t + w) // 16].view(torch.uint8), c.k_scale[:, :, b], c.v_scale[:, :, b]]
+
+    def mark(self) -> None:
+        self._marked = self.n
+        self._open = [x.clone() for x in self._block_at(self.n)] if self.n % self.block else None
+        if self._rows is None:
+            self._rows = torch.empty(len(self.P.layers), self.few_rows, 3 * self.P.d, dtype=BF16, device=self.device)
+
+    def truncate(self, n: int) -> None:
+        """... Up to few_rows rows behind the last mark() can be dropped, or whole blocks: anything else would leave its traces in the scales."""
+        assert 0 <= n <= self.n, f"truncate({n}) of {self.n} positions"
+        b0 = n // self.block * self.block
+        if b0 < n < self.n:
+            m = self._marked
+            if m is None or n < m:
+                raise ValueError(f"KV8Decoder: the rows from {n} on share a block of {self.block} positions with older ones and no mark() stands before them")
+            if b0 < m:
+                for x, old in zip(self._block_at(n), self._open):
+                    x.copy_(old)
+            first, L, c = max(m, b0), len(self.P.layers), self.cache
+            at = torch.arange(first, n, dtype=torch.int32, device=self.device).unsqueeze(1).expand(-1, L).contiguous()
+            x = self._rows.view(L, self.few_rows, 3, c.heads, c.hd)
+            for i in range(n - first):
+                r = slice(first - m + i, first - m + i + 1)
+                ops.kv8_append(c, x[:, r, 1], x[:, r, 2], at[i])
+        super().truncate(n)
+
+    def _next_rows(self, n: int) -> None:
+        if self._marked is not None:
+            if self.n - self._marked + n > self.few_rows:
+                self._marked = None
+            else:
+                self._at = self.pos + self._steps[:n]
+
+    def _qkv_rows(self, li: int, n: int) -> torch.Tensor:
+        if self._marked is None:
+            return super()._qkv_rows(li, n)
+        j = self.n - self._marked
+        return self._rows[li, j:j + n]
 
     def _attend_few(self, li: int, rows: torch.Tensor, o: torch.Tensor) -> None:
-        H, c = self.P.heads, self.caches[li]
-        x = rows.view(1, rows.shape[0], 3, H, c.hd)
-        ops.kv8_append(c, x[:, :, 1], x[:, :, 2], self.pos)
-        ops.attn_kv8(c, x[:, :, 0], self.pos, window=self.window, sinks=self.sinks, out=o.view(1, rows.shape[0], H, c.hd))
+        n, H, c = rows.shape[0], self.P.heads, self.caches[li]
+        x, out = rows.view(1, n, 3, H, c.hd), o.view(1, n, H, c.hd)
+        calls = [(slice(0, n), self.pos)] if self._marked is None else [(slice(i, i + 1), self._at[i:i + 1]) for i in range(n)]
+        for r, pos in calls:
+            ops.kv8_append(c, x[:, r, 1], x[:, r, 2], pos)
+            ops.attn_kv8(c, x[:, r, 0], pos, window=self.window, sinks=self.sinks, out=out[:, r])
 
     def _project_attend(self, li: int, lp: LayerParams, a1: torch.Tensor, n0: int, T: int) -> torch.Tensor:
         d, n = self.P.d, T - n0
-        qkv = torch.empty(n, 3 * d, dtype=BF16, device=a1.device)
-        ops.gemm(a1, lp.w_qkv, n, 3 * d, d, b_kstrided=True, bias=lp.b_qkv, out_bf16=qkv)
+        qkv = self._qkv_rows(li, n)
+        ops.gemm(a1, lp.w_qkv, n, 3 * d, d, b_kstrided=True, bias=lp.b_qkv, out_bf16=qkv, ldcb=3 * d)
         o = torch.empty(n, d, dtype=BF16, device=a1.device)
         self._attend_few(li, qkv, o)
         return o

@@ -858,7 +858,8 @@ class GatoPolicy(nn.Module):
     def predict_text_speculative(self, batch_dict, draft: "GatoPolicy", max_length=20, deterministic=True, n_draft=4, temperature=1.0, generator=None):
         """predict_text with `draft` -- a smaller policy over the same vocabulary -- proposing n_draft tokens at a time and this policy judging them
         in one step of n_draft + 1 rows (ops.verify_draft): greedy, the tokens are this policy's own best ones; sampled, they follow its
-        softmax at `temperature` exactly, whatever the draft proposes.  Same return value as predict_text.  Prompt, answer and drafts
+        softmax at `temperature`, whatever the draft proposes (an 8-bit cache takes drafted rows one at a time and forgets dropped ones without a
+        trace, so the logits that judge a token are the plain decode step's).  Same return value as predict_text.  Prompt, answer and drafts
         have to fit in context_len (nothing is cut on the left here)."""
         if not 1 <= n_draft <= 7:
             raise ValueError("n_draft must be 1 .. 7 (a judging step takes up to 8 rows)")
@@ -897,13 +898,16 @@ class GatoPolicy(nn.Module):
             proposed, dl = [], []
             nxt = torch.tensor(feed, device=dev)
             base_t, base_d = tgt.n, drf.n + len(feed)
-            for _ in range(n_draft):
+            for i in range(n_draft):
                 lg = rows(1, drf.extend(tables[1].index_select(0, nxt + lo))[-1:])
+                if i == 0:
+                    drf.mark()
                 nxt = pick(lg).reshape(1)
                 proposed.append(nxt)
                 dl.append(lg)
             x = torch.cat(proposed)
             judged = torch.cat([torch.tensor(tokens[-1:], device=dev), x])
+            tgt.mark()
             lt = rows(0, tgt.extend(tables[0].index_select(0, judged + lo)))             # row i: the distribution of proposed token i
             if deterministic:
                 acc, out = ops.verify_draft(lt.unsqueeze(0), x.reshape(1, -1), temperature=0.0)
