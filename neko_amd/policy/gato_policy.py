@@ -776,21 +776,30 @@ class GatoPolicy(nn.Module):
     # window is truncated on the left and RE-PRIMED (every remaining row recomputed without the dropped ones, exactly
     # what a full forward over the truncated window computes).  Pinned by fixture G12 (tests/golden/
     # make_fixture_decode.py: the reference's own predict_text / predict_response / predict_control outputs).
-    def _new_decoder(self, cap: int, device) -> "engine.KVDecoder":
-        sp = self.transformer._stack_params()
-        if self.kv_cache == "bf16":
-            if self.decode_window:
-                raise ValueError("decode_window needs kv_cache = 'e4m3' or 'int8'")
-            return engine.KVDecoder(sp, cap, device)
-        kinds = {"e4m3": torch.float8_e4m3fn, "int8": torch.int8}
+    def _cache_dtype(self) -> torch.dtype:
+        """What kv_cache stands for; raises for settings of the decode caches that do not go together (asked before a cached decoder is looked up)."""
+        kinds = {"bf16": torch.bfloat16, "e4m3": torch.float8_e4m3fn, "int8": torch.int8}
         if self.kv_cache not in kinds:
             raise ValueError(f"kv_cache must be 'bf16', 'e4m3' or 'int8', got {self.kv_cache!r}")
-        return engine.KV8Decoder(sp, cap, device, dtype=kinds[self.kv_cache], window=self.decode_window, sinks=self.decode_sinks)
+        if self.decode_window < 0 or self.decode_sinks < 0:
+            raise ValueError("decode_window and decode_sinks must not be negative")
+        if self.decode_window and self.kv_cache == "bf16":
+            raise ValueError("decode_window needs kv_cache = 'e4m3' or 'int8'")
+        if self.decode_sinks and not self.decode_window:
+            raise ValueError("decode_sinks need decode_window (without one every position stays visible)")
+        return kinds[self.kv_cache]
+
+    def _new_decoder(self, cap: int, device) -> "engine.KVDecoder":
+        sp, dtype = self.transformer._stack_params(), self._cache_dtype()
+        if dtype == torch.bfloat16:
+            return engine.KVDecoder(sp, cap, device)
+        return engine.KV8Decoder(sp, cap, device, dtype=dtype, window=self.decode_window, sinks=self.decode_sinks)
 
     def _decode_tokens(self, token_embeddings, n_tokens, start_token, end_token, deterministic):
         """Autoregressive continuation of ONE unpadded sequence.  Returns (logits (n_tokens, end-start+1) fp32,
         list of 0-d token tensors in the global vocabulary)."""
         assert token_embeddings.shape[0] == 1, "decode works on a single sequence"
+        self._cache_dtype()
         emb = token_embeddings[0, -self.context_len:, :].to(torch.float32)
         hp = self._head_params()
         self._flat.ensure_shadow()
