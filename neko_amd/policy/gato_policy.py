@@ -18,6 +18,7 @@ from __future__ import annotations
 from collections import OrderedDict
 from typing import List, Optional, Sequence, Union
 
+import math
 import os
 
 import numpy as np
@@ -423,6 +424,17 @@ class _StubTokenizer:
 
     def decode(self, ids):
         return " ".join(str(int(i)) for i in ids)
+
+
+def sample_token(logits: torch.Tensor, temperature: float, generator=None) -> torch.Tensor:
+    """0-d index drawn from softmax(logits / temperature) of one row: the weights (in 64 bits, the largest exactly 1 at any temperature) race against
+    exponential noise, as torch.multinomial's do -- whose check of the weights ends the process on the GPU when one is no number.  NaN counts as
+    -inf, infinite logits share the mass, and a row that holds neither gives any index."""
+    x = torch.nan_to_num(logits.double(), nan=-math.inf, posinf=math.inf, neginf=-math.inf)
+    m = x.max()
+    w = torch.where(x == m, 1.0, torch.exp((x - m) / temperature))
+    noise = torch.empty(x.shape, dtype=torch.float32, device=x.device).exponential_(1.0, generator=generator)
+    return torch.argmax(w / noise)
 
 
 class GatoPolicy(nn.Module):
@@ -874,8 +886,8 @@ class GatoPolicy(nn.Module):
             raise ValueError("n_draft must be 1 .. 7 (a judging step takes up to 8 rows)")
         if draft.vocab_size != self.vocab_size or draft.token_ends["text"] != self.token_ends["text"]:
             raise ValueError("the drafting policy must have the same vocabulary")
-        if not deterministic and not temperature > 0:
-            raise ValueError("temperature must be positive")
+        if not deterministic and not 0 < temperature <= torch.finfo(torch.float32).max:
+            raise ValueError("temperature must be positive and finite")
         if max_length < 1:
             raise ValueError("max_length must be positive")
         lo, hi = self.token_starts["text"], self.token_ends["text"]
@@ -896,9 +908,11 @@ class GatoPolicy(nn.Module):
         def pick(lg):           # (1, V) -> 0-d token within the text range
             if deterministic:
                 return torch.argmax(lg[0])
-            return torch.multinomial(torch.softmax(lg[0] / temperature, -1), 1, generator=generator)[0]
+            return sample_token(lg[0], temperature, generator)
 
         first = rows(0, tgt.extend(embs[0])[-1:])
+        if not bool((first > -math.inf).any()):
+            raise RuntimeError("the policy's logits hold no number: no token to go on with")
         drf.extend(embs[1])
         tok = pick(first)
         logits, tokens = [first[0]], [int(tok)]
