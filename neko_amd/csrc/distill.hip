@@ -262,12 +262,14 @@ __global__ __launch_bounds__(NT, NCH <= 7 ? 8 : NT == 512 ? 6 : 4) void distill_
 #pragma unroll 1
       for (int j = lane; j < a.k; j += 64) {
         const float t = __int_as_float(s_e[j].y);
-        if (t > 0.f) acc += t * ((s_z[j] - m) * c1);
+        if (t > 0.f) acc += t * (s_z[j] - m);
       }
     acc = wave_sum(acc);
     if (lane == 0) {
       float loss = 0.f;
-      if (soft) loss += soft_w * a.tau * a.tau * (s_teacher[0] + LN2 * (log2f(sum_soft) - acc));
+      // tau^2 (sum t log t + log sum - sum t (z - m) / tau), with one tau multiplied through: neither tau^2 nor (z - m) / tau is formed, which a
+      // small tau takes out of fp32
+      if (soft) loss += soft_w * a.tau * (a.tau * (s_teacher[0] + LN2 * log2f(sum_soft)) - acc);
       if (has_y) loss += a.hard * LN2 * (log2f(sum_hard) - (zy - m) * (TWO ? LOG2E : c1));
       a.loss_row[row] = loss;
     }
@@ -386,7 +388,7 @@ int launch(const DistillArgs& a, int R, hipStream_t s) {
 int neko_distill_topk_impl(const void* z, long ldz, int is_bf16, int R, int V, int Vpad, const float* t_val, const int* t_idx, int k, const float* weight,
                            float tau, const long long* target, float hard, float* loss_row, void* dlogits, long ldd, hipStream_t s) {
   if (!z || !weight || R <= 0 || V <= 0 || Vpad < V || (!loss_row && !dlogits)) return NEKO_ERR_ARG;
-  if (!(tau >= 1.17549435e-38f) || !(hard >= 0.f && hard <= 1.f) || (hard > 0.f && !target) || (hard < 1.f && (!t_val || !t_idx || k <= 0))) return NEKO_ERR_ARG;
+  if (!(tau >= 1.17549435e-38f && tau <= 3.402823466e38f) || !(hard >= 0.f && hard <= 1.f) || (hard > 0.f && !target) || (hard < 1.f && (!t_val || !t_idx || k <= 0))) return NEKO_ERR_ARG;
   if (k > KMAX) return NEKO_ERR_UNSUPPORTED;
   const int n = is_bf16 ? 8 : 4;
   if (Vpad % n || ldz % n || ldz < Vpad || (uintptr_t)z & 15) return NEKO_ERR_ARG;
