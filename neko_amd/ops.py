@@ -665,10 +665,16 @@ class KV8Cache:
         self._set(u8[0].view(dtype), u8[1].view(nseq, heads, cap // 16, hd, 16).view(dtype), sc[0], sc[1], nseq, heads, cap, hd, block)
 
     def _set(self, k, v, k_scale, v_scale, S, H, cap, hd, block):
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.nseq, self.heads, self.cap, self.hd, self.block, self.dtype = S, H, cap, hd, block, k.dtype
         # the leading arguments of every entry point of the cache
-        self._args = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), _KV8_DTYPES[k.dtype], S, H, cap, hd, block)
+        args = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), _KV8_DTYPES[k.dtype], S, H, cap, hd, block)
+        for put, value in zip(_KV8_PUT, (k, v, k_scale, v_scale, S, H, cap, hd, block, k.dtype, args)):
+            put(self, value)
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"KV8Cache.{name} stays what it is (its address and sizes are checked once): copy into the tensor, or make another cache")
+
+    def __reduce__(self):                 # copies and pickles: over their own tensors
+        return KV8Cache.from_tensors, (self.k, self.v, self.k_scale, self.v_scale)
 
     @property
     def device(self) -> torch.device:
@@ -710,6 +716,9 @@ class KV8Cache:
         p = x.data_ptr()
         assert (st | ss) % 8 == 0 and p % 16 == 0, f"{name}: rows must be 16-byte aligned"
         return T, ss, st, p
+
+
+_KV8_PUT = [getattr(KV8Cache, name).__set__ for name in KV8Cache.__slots__]       # (past __setattr__)
 
 
 def kv8_append(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, n_new: Optional[torch.Tensor] = None) -> None:
