@@ -388,7 +388,7 @@ int neko_patch_pos_add_bwd_sorted(const float* dout, const int* hkeys_sorted, co
  *   indices (t_val, t_idx [R][k]; an index outside [0, V) is no entry; equal indices add up):
  *     loss_row = (1 - hard) tau^2 KL(softmax(t / tau) || softmax(z / tau)) + hard CE(z, target)      (target int64 [R], < 0: no such term)
  *     dlogits  = weight[r] d loss_row / dz in z's type, 0 in columns V .. Vpad-1; may be z itself; NULL: loss only
- *   weight 0: loss 0, gradient 0.  k <= 1024; Vpad, ldz, ldd multiples of 16 bytes; tau finite, at least the smallest normal number.  Rows of dlogits that
+ *   weight 0: loss 0, gradient 0.  k <= 1024; Vpad <= 2^30; Vpad, ldz, ldd multiples of 16 bytes; tau finite, at least the smallest normal number.  Rows of dlogits that
  *   overlap z in part are refused. */
 int neko_kv8_append(void* k8, void* v8, float* k_scale, float* v_scale, int dtype, int nseq, int H, int cap, int hd, int block, const uint16_t* k,
                     long k_ss, long k_st, const uint16_t* v, long v_ss, long v_st, const int* pos, const int* n_new, int T, void* stream);

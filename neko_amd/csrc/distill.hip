@@ -389,7 +389,7 @@ int neko_distill_topk_impl(const void* z, long ldz, int is_bf16, int R, int V, i
                            float tau, const long long* target, float hard, float* loss_row, void* dlogits, long ldd, hipStream_t s) {
   if (!z || !weight || R <= 0 || V <= 0 || Vpad < V || (!loss_row && !dlogits)) return NEKO_ERR_ARG;
   if (!(tau >= 1.17549435e-38f && tau <= 3.402823466e38f) || !(hard >= 0.f && hard <= 1.f) || (hard > 0.f && !target) || (hard < 1.f && (!t_val || !t_idx || k <= 0))) return NEKO_ERR_ARG;
-  if (k > KMAX) return NEKO_ERR_UNSUPPORTED;
+  if (k > KMAX || Vpad > (1 << 30)) return NEKO_ERR_UNSUPPORTED;        // (columns and a workgroup's width add up in 32 bits)
   const int n = is_bf16 ? 8 : 4;
   if (Vpad % n || ldz % n || ldz < Vpad || (uintptr_t)z & 15) return NEKO_ERR_ARG;
   if (dlogits && (ldd % n || ldd < Vpad || (uintptr_t)dlogits & 15)) return NEKO_ERR_ARG;

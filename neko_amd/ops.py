@@ -611,6 +611,7 @@ def patch_pos_add_bwd(dout, hpos, wpos, d_row, d_col, sorted_rows=None):
 # detailed message is worked out only when it fails), memoised workspace sizes (functions of the sizes alone), entry points bound once.
 _KV8_DTYPES = {torch.float8_e4m3fn: 0, torch.int8: 1}
 _I32, _I64, _F32 = torch.int32, torch.int64, torch.float32
+_MAX_COLS = 1 << 30                  # logits of a row (columns are 32-bit integers in the kernels, and sums of them with a workgroup's width)
 
 
 def _here(t: torch.Tensor, name: str) -> int:
@@ -760,6 +761,7 @@ def attn_kv8(cache: KV8Cache, q: torch.Tensor, pos: torch.Tensor, n_new: Optiona
     assert T <= cap, "more rows than the cache has positions"
     assert window >= 0 and sinks >= 0 and (sinks == 0 or window > 0), "sinks need a window"
     assert scale is None or scale > 0.0, "scale must be positive"
+    window, sinks, max_len = min(window, cap), min(sinks, cap), min(max_len, cap)       # no more than everything (and within 32 bits)
     if out is None:
         out = torch.zeros((S, T, HG, hd), dtype=BF16, device=cache.device)          # (positions outside the cache are no rows of the call either)
     To, o_ss, o_st, op = cache.row_strides(out, HG, "out", dev)
@@ -795,7 +797,8 @@ def verify_draft(logits: torch.Tensor, tokens: torch.Tensor, draft_logits: Optio
     B, K = tokens.shape
     assert B > 0 and 0 < K <= 62, "1 to 62 drafted tokens"
     V = logits.shape[-1]
-    assert V > 0 and temperature >= 0.0, "temperature must not be negative"
+    assert 0 < V <= _MAX_COLS, f"1 to {_MAX_COLS} logits a row"
+    assert temperature >= 0.0, "temperature must not be negative"
     dev = _here(logits, "logits")
     tp, t_sb, t_sr = _logit_rows(logits, (B, K + 1, V), "logits", dev)
     dp, d_sb, d_sr = None, 0, 0
@@ -829,6 +832,7 @@ def distill_topk(z: torch.Tensor, V: int, Vpad: int, t_val: Optional[torch.Tenso
     assert z.dtype is _F32 or z.dtype is BF16, f"z must be float32 or bfloat16, got {z.dtype}"
     assert z.dim() == 2 and z.shape[1] >= Vpad >= V > 0 and z.stride(1) == 1, "z must be [R, >= Vpad] with contiguous rows"
     R = z.shape[0]
+    assert Vpad <= _MAX_COLS and R < 2 ** 31, f"at most {_MAX_COLS} columns and 2^31 - 1 rows"
     assert R > 0 and tau > 0.0 and 0.0 <= hard <= 1.0, "tau must be positive, hard in [0, 1]"
     assert loss_row is not None or dlogits is not None, "nothing to compute"
     k, tv, ti = 0, None, None
