@@ -157,6 +157,14 @@ def collect_sources(inputs: Sequence[dict]) -> PackedBatch:
     return pb
 
 
+def check_positions(desc: np.ndarray, pos_rows: int) -> None:
+    """Local positions index the position table on the device without a test of their own: a layout that leaves it is refused here, as the
+    reference's nn.Embedding does (gato_policy.py:380-385)."""
+    top = int(desc[:, 2].max()) if desc.shape[0] else -1
+    if top >= pos_rows:
+        raise ValueError(f"a timestep has {top + 1} observation tokens, the position table (context_len) {pos_rows} rows")
+
+
 def build_layout(inputs: Sequence[dict], use_pos_encoding: bool, context_len: int, pad_seq: bool,
                  n_patches_of=None, ragged_groups: int = 0) -> PackedBatch:
     """Turn the list of example dicts into one descriptor table + source lists (host only, numpy).
@@ -543,8 +551,9 @@ class GatoPolicy(nn.Module):
         self.last_pack: Optional[_PackInfo] = None      # statistics of the last packed batch (bench / logging only)
         #: what the decode helpers keep keys and values in: "bf16", or "e4m3" / "int8" with a scale per 32 positions and head (engine.KV8Decoder)
         self.kv_cache = os.environ.get("NEKO_KV_CACHE", "bf16")
-        #: > 0 (8-bit caches only): a decoded row sees the last decode_window positions and the first decode_sinks, and a sequence that outgrows
-        #: context_len goes on instead of being cut on the left and recomputed
+        #: > 0 (8-bit caches only): a decoded row sees the last decode_window positions and the first decode_sinks; in predict_text and predict_control
+        #: a sequence that outgrows context_len then goes on instead of being cut on the left and recomputed (a longer prompt is still cut to
+        #: its last context_len positions).  predict_response and predict_text_speculative end at context_len with it as without
         self.decode_window, self.decode_sinks = 0, 0
         self._dp = None
         self._layout_cache: "OrderedDict" = OrderedDict()      # structural memo of _prepare (layout_signature)
@@ -647,6 +656,7 @@ class GatoPolicy(nn.Module):
             pb.B, pb.T, pb.segments, pb.order = hit.B, hit.T, hit.segments, hit.order
         else:
             pb = build_layout(inputs, self.use_pos_encoding, self.context_len, self.pad_seq, ragged_groups=ragged_groups)
+            check_positions(pb.desc, pos_rows)
         has_text = hit.has_text if hit is not None else bool(np.isin(pb.desc[:, 0], (K_TOKEN, K_DEVID)).any())
         if self._dp is not None and getattr(self._dp, "no_text_declared", False) and has_text:
             raise RuntimeError("text tokens in a batch, but the data-parallel reducer was told that the text rows of "
@@ -972,14 +982,14 @@ class GatoPolicy(nn.Module):
         n_patches = image_embeddings.shape[1]
         pred_logits, response_tokens = [], []
         for idx in range(max_length):
-            batch_dict = {"image_embeddings": image_embeddings, "text": torch.tensor(prompt_tokens + response_tokens)}
-            emb, _, _, _ = self.tokenize_input_dicts([batch_dict])
             n_seq = n_patches + len(prompt_tokens) + idx          # positions before the separator
-            rows = emb[0, :n_seq, :].to(torch.float32)
-            if n_seq > self.context_len:
+            if n_seq > self.context_len:                          # (a window changes nothing: the position table ends there)
                 raise ValueError("predict_response: sequence exceeds context_len")
             if n_seq == 0:
                 raise ValueError("predict_response needs at least one position (image or prompt)")
+            batch_dict = {"image_embeddings": image_embeddings, "text": torch.tensor(prompt_tokens + response_tokens)}
+            emb, _, _, _ = self.tokenize_input_dicts([batch_dict])
+            rows = emb[0, :n_seq, :].to(torch.float32)
             h = dec.extend(rows[dec.n:])
             nxt = engine.lm_head_rows(hp, h[-1:])[0, start_token:(end_token + 1)]
             if deterministic:
