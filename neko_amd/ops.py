@@ -842,13 +842,13 @@ def distill_topk(z: torch.Tensor, V: int, Vpad: int, t_val: Optional[torch.Tenso
         assert 0 < k <= 1024, "1 to 1024 teacher entries"
         tv, ti = _vec(t_val, R * k, "t_val", dev, _F32), _vec(t_idx, R * k, "t_idx", dev)
     assert hard == 0.0 or target is not None, "hard > 0 needs target"
-    ldz, ldd, dp = (z.stride(0) if R > 1 else z.shape[1]), 0, None
+    ldz, ldd, dp = (z.stride(0) if R > 1 else Vpad), 0, None        # (a single row has no stride)
     if dlogits is not None:
         if dlogits.get_device() != dev or dlogits.dtype is not z.dtype:
             _here(dlogits, "dlogits")
         assert dlogits.dtype is z.dtype and dlogits.dim() == 2 and dlogits.shape[0] == R and dlogits.shape[1] >= Vpad and dlogits.stride(1) == 1, \
             "dlogits must be like z"
-        ldd, dp = (dlogits.stride(0) if R > 1 else dlogits.shape[1]), dlogits.data_ptr()
+        ldd, dp = (dlogits.stride(0) if R > 1 else Vpad), dlogits.data_ptr()
     rc = _entry("neko_distill_topk")(z.data_ptr(), ldz, z.dtype is BF16, R, V, Vpad, tv, ti, k, _vec(weight, R, "weight", dev, _F32), tau,
                                      _vec(target, R, "target", dev, _I64), hard, _vec(loss_row, R, "loss_row", dev, _F32), dp, ldd, _raw(dev))
     if rc:

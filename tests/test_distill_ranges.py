@@ -61,3 +61,18 @@ def test_long_rows(V, tau, hard, dtype):
     out_round = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24
     fold = 2.0 ** -18 if dtype == torch.bfloat16 else 0.0                  # the folded factor's logarithm in the exponent (below 64 in size)
     assert bool(((dz[:, :V].double() - rg).abs() <= out_round * rg.abs() + (2 * rel + fold) * mag + 1e-38).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_single_row_of_any_width(dtype):
+    """One row beside others' columns: there is no stride to be a multiple of 16 bytes, and columns behind Vpad stay."""
+    from neko_amd import ops
+    z, Vpad, tv, ti, w, y = _case(1, 300, 5, dtype, seed=1)
+    loss, dz = _run(z, 300, Vpad, tv, ti, w, y, 2.0, 0.3)
+    for extra in (1, 3, 16):
+        wide = torch.full((1, Vpad + extra), 5.0, dtype=dtype, device="cuda")
+        wide[:, :Vpad] = z.cuda()
+        out, l2 = torch.full_like(wide, 7.0), torch.empty(1, device="cuda")
+        ops.distill_topk(wide, 300, Vpad, tv.cuda(), ti.cuda(), w.cuda(), tau=2.0, target=y.cuda(), hard=0.3, loss_row=l2, dlogits=out)
+        assert torch.equal(l2.cpu(), loss) and torch.equal(out[:, :Vpad].cpu(), dz) and bool((out[:, Vpad:] == 7).all())
