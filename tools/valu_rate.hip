@@ -1,5 +1,5 @@
 // Issue-rate microbenchmark for the VALU instructions the attention / epilogue bodies are made of (gfx950).
-//   hipcc -O3 --offload-arch=gfx950 tools/valu_rate.hip -o /tmp/valu_rate && /tmp/valu_rate
+//   hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/valu_rate.hip -o /tmp/valu_rate && /tmp/valu_rate
 // Every kernel runs NW waves per SIMD on every CU, each wave issuing REP x 64 independent instructions of one kind;
 // cycles per instruction per SIMD = s_memtime ticks of a wave / (REP * 64) / waves-per-SIMD ... reported both as the
 // per-wave figure (latency-bound when 1 wave) and the per-SIMD throughput figure (4 waves per SIMD).
@@ -16,8 +16,6 @@ template <int KIND>
 __global__ __launch_bounds__(256) void k(float* out, long long* cyc, float seed) {
   float a0 = seed + threadIdx.x, a1 = a0 + 1, a2 = a0 + 2, a3 = a0 + 3, a4 = a0 + 4, a5 = a0 + 5, a6 = a0 + 6, a7 = a0 + 7;
   float b0 = 1.0001f, b1 = 0.5f;
-  typedef float f2 __attribute__((ext_vector_type(2)));
-  f2 p0 = {a0, a1}, p1 = {a2, a3}, p2 = {a4, a5}, p3 = {a6, a7}, q = {b0, b1};
   unsigned u0 = threadIdx.x * 2654435761u, u1 = u0 ^ 0x1234567u;
   __syncthreads();
   const long long t0 = __builtin_readcyclecounter();
@@ -26,9 +24,6 @@ __global__ __launch_bounds__(256) void k(float* out, long long* cyc, float seed)
     if (KIND == 0) {   // v_fma_f32, 8 independent chains
       asm volatile(BODY16("v_fma_f32 %0, %0, %8, %9\n v_fma_f32 %1, %1, %8, %9\n v_fma_f32 %2, %2, %8, %9\n v_fma_f32 %3, %3, %8, %9\n")
                    : "+v"(a0), "+v"(a1), "+v"(a2), "+v"(a3), "+v"(a4), "+v"(a5), "+v"(a6), "+v"(a7) : "v"(b0), "v"(b1));
-    } else if (KIND == 1) {   // v_pk_fma_f32
-      asm volatile(BODY16("v_pk_fma_f32 %0, %0, %4, %4\n v_pk_fma_f32 %1, %1, %4, %4\n v_pk_fma_f32 %2, %2, %4, %4\n v_pk_fma_f32 %3, %3, %4, %4\n")
-                   : "+v"(p0), "+v"(p1), "+v"(p2), "+v"(p3) : "v"(q));
     } else if (KIND == 2) {   // v_exp_f32
       asm volatile(BODY16("v_exp_f32 %0, %0\n v_exp_f32 %1, %1\n v_exp_f32 %2, %2\n v_exp_f32 %3, %3\n")
                    : "+v"(a0), "+v"(a1), "+v"(a2), "+v"(a3));
@@ -44,9 +39,6 @@ __global__ __launch_bounds__(256) void k(float* out, long long* cyc, float seed)
     } else if (KIND == 6) {   // v_cndmask_b32 (vcc)
       asm volatile(BODY16("v_cndmask_b32 %0, %4, %5, vcc\n v_cndmask_b32 %1, %5, %6, vcc\n v_cndmask_b32 %2, %6, %7, vcc\n v_cndmask_b32 %3, %7, %4, vcc\n")
                    : "+v"(a0), "+v"(a1), "+v"(a2), "+v"(a3) : "v"(a4), "v"(a5), "v"(a6), "v"(a7) : "vcc");
-    } else if (KIND == 7) {   // v_pk_mul_f32
-      asm volatile(BODY16("v_pk_mul_f32 %0, %0, %4\n v_pk_mul_f32 %1, %1, %4\n v_pk_mul_f32 %2, %2, %4\n v_pk_mul_f32 %3, %3, %4\n")
-                   : "+v"(p0), "+v"(p1), "+v"(p2), "+v"(p3) : "v"(q));
     } else if (KIND == 8) {   // v_add_f32
       asm volatile(BODY16("v_add_f32 %0, %0, %4\n v_add_f32 %1, %1, %4\n v_add_f32 %2, %2, %4\n v_add_f32 %3, %3, %4\n")
                    : "+v"(a0), "+v"(a1), "+v"(a2), "+v"(a3) : "v"(b0));
@@ -90,7 +82,7 @@ __global__ __launch_bounds__(256) void k(float* out, long long* cyc, float seed)
   }
   const long long t1 = __builtin_readcyclecounter();
   if (threadIdx.x % 64 == 0) cyc[blockIdx.x * (blockDim.x / 64) + threadIdx.x / 64] = t1 - t0;
-  out[blockIdx.x * blockDim.x + threadIdx.x] = a0 + a1 + a2 + a3 + a4 + p0[0] + p1[1] + p2[0] + p3[1] + (float)(u0 + u1);
+  out[blockIdx.x * blockDim.x + threadIdx.x] = a0 + a1 + a2 + a3 + a4 + (float)(u0 + u1);
 }
 
 template <int KIND>
@@ -125,8 +117,6 @@ void run(const char* name, int waves_per_simd) {
 int main() {
   for (int w : {1, 4}) {
     run<0>("v_fma_f32", w);
-    run<1>("v_pk_fma_f32", w);
-    run<7>("v_pk_mul_f32", w);
     run<8>("v_add_f32", w);
     run<2>("v_exp_f32", w);
     run<10>("v_rcp_f32", w);
