@@ -373,6 +373,8 @@ int neko_patch_pos_add_bwd_sorted(const float* dout, const int* hkeys_sorted, co
  * neko_attn_kv8: T rows a sequence at positions pos[s] + i (i < n as above; other rows of `out` are left as they are), G query heads per key
  *   head (query head h * G + g reads key head h), q and out bf16 with strides as k above.  Row at position p sees t with start[s] <= t <= p and,
  *   where window > 0, t > p - window or t < start[s] + sinks (start NULL: 0).  A row that sees nothing is 0.  `scale` > 0 multiplies q . k.
+ *   Scores and sums are fp32; the probabilities enter the product with the values as two bf16 (16 bits) where T * G <= 64, above as one bf16
+ *   (half a step of 2^-8, averaged over the keys: 0.0018 instead of 0.0016 relative to a 64-bit result that is rounded to bf16).
  *   `out` may be q itself, rows beside q's in one buffer or memory of its own; rows that overlap otherwise are refused.  Scores are held for
  *   |scale q . k| up to 2^29, values up to the largest the cache keeps (beside a value of more than 2^40, one smaller by 2^160 may count as 0).
  *   What lies in the cache outside [start, last row] never reaches the output.  max_len: host-known bound on pos + T (0: cap); it sizes

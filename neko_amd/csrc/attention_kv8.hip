@@ -329,8 +329,8 @@ __global__ __launch_bounds__(NW * 64, NQ == 1 || HD < 128 ? 2 : 1) void attn_kv8
 // factor), so the common step takes no maximum.  Probabilities are rounded to bf16 once, and the sums are of the rounded ones: their errors are
 // independent and average out like the values' own (measured 1.0-1.4 x the error of the rounded output); a second product for their low parts
 // would cost 50 % of the matrix work.
-// 4 sequences x 16 heads of 128, 1024 queries over 2976-4000 keys: 126 us in a row of calls (0.93 PFLOP/s), 140 one at a time (156 with a maximum
-// a tile).  The products and their operand reads alone take 53 us, with the staging 62: what binds it are
+// 4 sequences x 16 heads of 128, 1024 queries over 2976-4000 keys: 127-133 us in a row of calls (0.88-0.92 PFLOP/s), 140-150 one at a time (156 with a
+// maximum a tile).  The products and their operand reads alone take 53 us, with the staging 62: what binds it are
 // the vector instructions of the softmax (130 a tile and wave), which two waves of a SIMD in the same phase do not hide behind each other's
 // products.  Opposite phases for the two halves of the workgroup, a barrier between the phases, took 151; softmax of one tile beside the products
 // of another within a wave 155, and so with 64 rows a wave, one wave per SIMD, 176.

@@ -8,10 +8,11 @@
 //
 // Bound by HBM: V logits in, V gradients out (the softmax needs the whole row before the first gradient, so the row stays in registers
 // between the two: up to 1024 threads x 13 pieces of 16 B; longer rows are read again, from the last-level cache).  8192 rows of 52305 bf16 logits
-// at two temperatures, a tenth of them of weight 0: 375 us, 1.63 GB at 4.4 TB/s (a copy reaches 5.2).  The k + 1 sparse places are
+// at two temperatures, a tenth of them of weight 0: 368 us, 1.63 GB at 4.4 TB/s (a copy reaches 5.2).  The k + 1 sparse places are
 // written a second time behind the dense pass, with the dense term formed again from the logit that the thread kept: equal indices add up in
-// registers (every holder writes the same sum), so no atomics and one rounding per element.  Sums are fp32 of at most 52 K positive terms in
-// a tree (a thread's 56, then lanes, then waves).  dlogits may be z.
+// registers (every holder writes the same sum), so no atomics and one rounding per element.  Sums are fp32 of positive terms: a thread adds its
+// pieces' one after the other (13 pieces of 8 bf16: 104; of a row that is read again, as many as it has, 152 in 150000 bf16 logits), then six levels
+// of lanes, then up to sixteen waves.  dlogits may be z.
 #include "neko_kernels.h"
 
 namespace {
@@ -335,7 +336,9 @@ __global__ __launch_bounds__(NT, NCH <= 7 ? 8 : NT == 512 ? 6 : 4) void distill_
 
 // Threads and rounds (pieces of 16 B a thread) by the pieces of a row: as many rounds as the row has, or little more -- a round computes whether the
 // row reaches it or not (a test per round cost more: it kept the rounds from overlapping) -- and workgroups as small as the registers allow, so that
-// several rows per CU fill each other's gaps.  Measured at 0.27-0.54 GB of bf16 | fp32 in and out, us:
+// several rows per CU fill each other's gaps.  A few of the variants at two temperatures in bf16 (512 threads, 11 to 14 rounds) keep 2 to 11 registers
+// in scratch (12-40 B a lane; one temperature, 1024 x 7: 2), and still are the fastest for their rows.  Measured in bf16 | fp32, us (in and out 0.37 | 0.37 GB at 700
+// pieces, 0.68 | 0.68 at 1300, 1.07 | 1.57 at 3000, 1.07 | 2.15 above):
 //   700 pieces:  256 threads 76 | 73, 512 threads 112 | 98          1300: 512 x 4 155 | 136, 1024 x 4 276 | 234        3000: 512 x 6 193 | 303, 1024 x 4 227 | 316
 //   5000: 1024 x 5 190 | 379, 512 x 10 200 | 397; at two temperatures in bf16, where registers for two rows more pay, 512 x 10 211, 1024 x 5 214
 //   6544: 1024 x 7 194 | 372, 512 x 13 206 | 401; two temperatures in bf16 512 x 13 234, 1024 x 7 247

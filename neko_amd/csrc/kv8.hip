@@ -15,8 +15,10 @@
 // bytes are contiguous instead, so the codes change hands through LDS: written and read there in the lane's own order, moved to and from
 // memory as consecutive 16-byte pieces (as 8-byte rows and 16-byte pieces 128 B apart they were 3 x the requests).  A piece belongs to
 // one lane: a partly filled one is read, changed and written by its owner.
-// 64 sequences of up to 1024 rows x 24 heads of 32, K and V: append 41-54 us (151 MB: 2.8-3.7 TB/s; ragged positions, so that most units begin and
-// end inside a block), read back 45 us (272 MB: 6.0 TB/s, codes partly out of the last-level cache; a copy reaches 5.2).
+// 64 sequences of up to 1024 rows x 24 heads of 32, K and V: append 42-53 us (151 MB: 2.8-3.6 TB/s), read back 45 us (272 MB: 6.0 TB/s, codes partly
+// out of the last-level cache; a copy reaches 5.2).  What keeps the append from the copy's rate are its registers: sixteen rows in flight and their
+// codes take 154-156 (int8 141-142), three waves per SIMD, where the read back has 52-60.  (Units that begin or end inside a block, and are read,
+// changed and written, are a few in a hundred there: two at most for a sequence and head.)
 #include "kv8.h"
 
 namespace {

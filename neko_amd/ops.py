@@ -751,8 +751,8 @@ def attn_kv8(cache: KV8Cache, q: torch.Tensor, pos: torch.Tensor, n_new: Optiona
              window: int = 0, sinks: int = 0, scale: Optional[float] = None, max_len: int = 0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of q [nseq, T, heads * G, hd] (bf16) at positions pos[s] + i over the cache (which holds those positions already: append
     first); causal, keys from start[s] on, optionally a sliding `window` with the first `sinks` keys kept visible.  Rows at and behind
-    n_new[s] of `out` are left as they are (a fresh output holds zeros there).  max_len: host-known bound on pos + T, sizes the launch.  See
-    neko_attn_kv8."""
+    n_new[s] of `out` are left as they are (a fresh output holds zeros there).  max_len: host-known bound on pos + T, sizes the launch.  Up to
+    64 rows a key head (T * G) the probabilities keep 16 bits, above 8.  See neko_attn_kv8."""
     dev = _here(cache.k, "cache")
     S, H, cap, hd = cache.nseq, cache.heads, cache.cap, cache.hd
     HG = q.shape[2] if q.dim() == 4 else 0
