@@ -668,10 +668,21 @@ class KV8Decoder(KVDecoder):
             for i in range(n - first):
                 r = slice(first - m + i, first - m + i + 1)
                 ops.kv8_append(c, x[:, r, 1], x[:, r, 2], at[i])
+        if self._marked is not None and n < self._marked:
+            self._marked = None
         super().truncate(n)
+
+    def capture_greedy_step(self, Hp: "HeadParams", table: torch.Tensor, start: int, end: int) -> None:
+        self._marked = None
+        super().capture_greedy_step(Hp, table, start, end)
+
+    def replay_greedy_step(self):
+        self._marked = None                       # (the captured step keeps no rows for truncate)
+        return super().replay_greedy_step()
 
     def _next_rows(self, n: int) -> None:
         if self._marked is not None:
+            assert self.n >= self._marked, "a mark behind the last row"
             if self.n - self._marked + n > self.few_rows:
                 self._marked = None
             else:

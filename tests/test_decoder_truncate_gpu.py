@@ -118,3 +118,41 @@ def test_drafted_decoding_does_not_depend_on_the_draft(kind):
         got, t = m.predict_text_speculative(_prompt(25), draft, max_length=30, n_draft=n_draft)
         assert [int(x) for x in t] == [int(x) for x in tokens]
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+def test_a_mark_ends_where_rows_before_it_go(kind):
+    """Whole blocks dropped from before a mark take the mark with them: rows that follow are ordinary ones."""
+    a, b = _decoders(kind)
+    for dec in (a, b):
+        dec.extend(_rows(40, 64, 0.0, 1))
+    a.mark()
+    a.extend(_rows(3, 64, 60.0, 2))
+    for dec in (a, b):
+        dec.truncate(32)
+        for n, seed in ((1, 3), (4, 4), (5, 5), (2, 6)):              # past the position that the mark stood at
+            h = dec.extend(_rows(n, 64, 0.5, seed))
+            assert bool(torch.isfinite(h.float()).all())
+    assert a.n == b.n == 44 and torch.equal(_held(a), _held(b))
+    with pytest.raises(ValueError, match="mark"):
+        a.truncate(41)
+
+
+def test_replayed_steps_end_a_mark():
+    """A captured step keeps no rows: what it appended cannot be dropped in part, and is what it would be without a mark."""
+    m = _policy(ctx=96)
+    m.kv_cache = "int8"
+    table, hp = m._flat.view("embed_token.weight"), m._head_params()
+    got = []
+    for marked in (False, True):
+        dec = m._new_decoder(96, torch.device(DEV))
+        dec.capture_greedy_step(hp, table, 0, 127)
+        dec.extend(m.tokenize_input_dicts([_prompt(20)])[0][0].float())
+        if marked:
+            dec.mark()
+        dec.g_x.copy_(table[5].reshape(1, -1))
+        out = [dec.replay_greedy_step() for _ in range(6)]
+        got.append((torch.stack([l for l, _ in out]), [int(t) for _, t in out], _held(dec)))
+        with pytest.raises(ValueError, match="mark"):
+            dec.truncate(22)
+    assert torch.equal(got[0][0], got[1][0]) and got[0][1] == got[1][1] and torch.equal(got[0][2], got[1][2])
