@@ -156,3 +156,15 @@ def test_replayed_steps_end_a_mark():
         with pytest.raises(ValueError, match="mark"):
             dec.truncate(22)
     assert torch.equal(got[0][0], got[1][0]) and got[0][1] == got[1][1] and torch.equal(got[0][2], got[1][2])
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("window,sinks", [(16, 4), (9, 0)])
+def test_drafted_decoding_under_a_window(kind, window, sinks):
+    """The same with a sliding window that leaves most of the sequence behind."""
+    m, draft = _policy(seed=0), _policy(seed=3, layers=1)
+    for p in (m, draft):
+        p.kv_cache, p.decode_window, p.decode_sinks = kind, window, sinks
+    want, tokens = m.predict_text(_prompt(35), max_length=30)
+    got, t = m.predict_text_speculative(_prompt(35), draft, max_length=30, n_draft=5)
+    assert [int(x) for x in t] == [int(x) for x in tokens] and torch.equal(got, want)
